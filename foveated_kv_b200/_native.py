@@ -44,6 +44,29 @@ class DecodeShape(C.Structure):
                 ("test_flags", C.c_int32)]
 
 
+class RotaryShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("B", "S", "Hq", "Hk", "D", "rot", "bf16", "interleaved",
+                                         "inverse", "pos64")] + \
+               [("amplitude", C.c_float), ("reserved", C.c_int32)] + \
+               [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "q_out_stride",
+                                             "k_out_stride")] + [("pos_stride", C.c_int64 * 2)]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k_pages", "v_pages", "k_scale", "v_scale", "table",
+                                          "lens", "status")] + \
+               [(n, C.c_int32) for n in ("B", "Hk", "D", "page", "n_pages", "width",
+                                         "table_stride", "fp8", "bf16", "reserved")]
+
+
+class PagedNew(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "q", "q_out", "cu_new", "inv_freq")] + \
+               [(n, C.c_int64 * 3) for n in ("k_stride", "v_stride", "q_stride",
+                                             "q_out_stride")] + \
+               [(n, C.c_int32) for n in ("T", "n_uniform", "Hq", "rot", "interleaved")] + \
+               [("amplitude", C.c_float)]
+
+
 FKV_TEST_STALL = 1
 FKV_ERR_TIMEOUT = -4
 
@@ -90,6 +113,11 @@ SIGNATURES = {
     "fkv_ipc_get_handle": (C.c_int, [P, P, C.POINTER(I64)]),
     "fkv_ipc_open": (C.c_int, [P, I64, C.POINTER(P)]),
     "fkv_ipc_close": (C.c_int, [P, I64]),
+    "fkv_rotary": (C.c_int, [C.POINTER(RotaryShape), P, P, P, P, P, P, P]),
+    "fkv_paged_append": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedNew), P]),
+    "fkv_paged_read": (C.c_int, [C.POINTER(PagedCache), I32, P, P, P]),
+    "fkv_paged_attend_workspace_bytes": (SZ, [C.POINTER(PagedCache), I32]),
+    "fkv_paged_attend": (C.c_int, [C.POINTER(PagedCache), I32, C.c_float, I32, P, P, P, P, SZ, P]),
     "fkv_promo_create": (P, [I32, I32, I32, I32]),
     "fkv_promo_register_archive": (C.c_int, [P, I32, C.c_char_p, C.c_char_p, I32, I32, I32,
                                              I32, P, I64]),

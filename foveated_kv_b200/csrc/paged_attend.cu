@@ -1,0 +1,860 @@
+// Attention of one new token per sequence over the paged cache, split over
+// the cache's length and joined (no counterpart in the reference, whose fused
+// decode wants every sequence of a batch to have one length).
+//
+//   out[h] = sum_n p_n v_n / sum_n p_n,  p_n = exp(scale q[h].k_n - m),
+//   n over the last `window` (or all) tokens of the sequence; a sequence
+//   without tokens gives zeros and a log-sum-exp of -inf.
+//
+// Work split.  A stream is one (sequence, kv head, tile of up to 8 NT query
+// heads); its tokens are cut into units of kUnit.  The units of all streams,
+// in order, are dealt to the CTAs of one wave in equal contiguous runs, so
+// every CTA reads the same number of bytes whatever the lengths are (the
+// lengths stay on the device: each CTA sums them up itself).  A CTA that
+// holds a whole stream writes its output; a piece of one is left as a record
+// (maximum, sum, unnormalised output) that a second, dependent launch joins.
+// No atomics and no counters: records and descriptors are written before they
+// are read in every call, so the workspace needs no initialisation, and two
+// calls share nothing.
+//
+// Tile.  One warp takes 16 tokens at a time straight from global memory to
+// registers, each lane in 16-byte pieces in the order in which the tensor
+// core wants them (row = lane / 4 = g, quad = lane % 4 = t):
+//   S^T (16 tok x 8 heads)  = K (16 x D) . Q^T      lane: rows g, g + 8 of K
+//   O^T (D x 8 heads)      += V^T (D x 16) . P^T    lane: rows 2t, 2t+1, 2t+8, 2t+9 of V
+// The products' inner order is free, so the 16-byte pieces of K pair with the
+// same pieces of Q; V rows pair up by byte permutes; P^T comes from S^T by an
+// 8x8 transpose across lanes.  K and V of the next tile are in flight while
+// this one is computed.
+//
+// 8-bit rows: codes become f16 exactly.  A key's scale multiplies its score.
+// A value's scale joins the exponent: w_n = exp2(x_n + log2 s_n - M) with a
+// running maximum M of its own, so w never leaves the range of f16 however
+// large or small the scales are, and the result is (sum w_n c_n) 2^(M-m) / l.
+#include <algorithm>
+#include <climits>
+#include <mutex>
+
+#include <cuda_fp8.h>
+
+#include "decode_common.cuh"
+#include "fkv_common.h"
+#include "paged.cuh"
+#include "rotary.cuh"
+
+using namespace fkvdev;
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr float kLazy = 8.f;          // log2 units a running maximum may lag behind
+
+enum { F16 = 0, BF16 = 1, FP8 = 2 };  // what the pages hold
+
+struct AttendArgs {
+    FkvPagedCache c;
+    const uint16_t* q;
+    uint16_t* out;
+    float* lse;
+    float* rec_o;      // (2 per CTA, 8 NT heads, D)
+    float4* rec_s;     // (2 per CTA, 8 NT heads): m, M, l
+    int4* desc;        // first output row, heads, pieces (0: nothing to join), first record
+    int Hq, G, HT, pshift, window, per_stream;
+    float sl2;         // scale * log2(e)
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^(a - b) where b is a maximum over a: 0 for an empty side
+__device__ __forceinline__ float ratio2(float a, float b) { return a == -INFINITY ? 0.f : ex2(a - b); }
+
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <bool BF>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    uint32_t b0, uint32_t b1) {
+    if (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int D, int KIND>
+struct Geo {
+    static constexpr int ES = KIND == FP8 ? 1 : 2;            // bytes of a stored element
+    // 16-token groups of one warp's tile
+    static constexpr int TG = D * ES >= 256 ? 1 : 2;
+    static constexpr int UNIT = kWarps * 16 * TG;             // tokens of one CTA step
+    static constexpr int KC = D * ES / 64;                    // 16-byte pieces of a key row per lane
+    static constexpr int KE = 16 / ES;                        // elements of a piece
+    static constexpr int KS = KE / 4;                         // tensor-core steps of a piece
+    static constexpr int VB = D * ES >= 128 ? 16 : 8;         // bytes of a value piece
+    static constexpr int VC = D * ES / (8 * VB);              // value pieces per lane and token
+    static constexpr int VW = VB / 4;                         // words of a value piece
+    static constexpr int VE = VB / ES;                        // elements of a value piece
+    static constexpr int MT = D / 16;                         // 16-row tiles of O^T
+};
+
+// CTAs per SM that a kernel's registers are held to
+template <int D, int NT>
+constexpr int kPerSm = D == 256 || NT == 2 ? 2 : 3;
+
+// Units of work of sequence b: tokens [lo, len), cut from lo rounded down to 16.
+__device__ __forceinline__ void seq_range(const AttendArgs& a, int b, int& lo, int& len) {
+    const int reach = a.c.width << a.pshift;
+    len = a.c.lens[b];
+    if (len > reach) {
+        paged_report(a.c.status, FKV_PAGED_BAD_POSITION);
+        len = reach;
+    }
+    len = max(len, 0);
+    lo = a.window > 0 ? max(0, len - a.window) : 0;
+}
+template <int UNIT>
+__device__ __forceinline__ int seq_units(int lo, int len) {
+    return len <= lo ? 0 : (len - (lo & ~15) + UNIT - 1) / UNIT;
+}
+
+template <int D, int NT, int KIND>
+struct Smem {
+    float o[kWarps][8 * NT][D + 2];
+    float m[kWarps][8 * NT], M[kWarps][8 * NT], l[kWarps][8 * NT];
+    int scan[kWarps];
+    int b, prefix, total;
+};
+
+template <int D, int NT, int KIND>
+__global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const __grid_constant__ AttendArgs a) {
+    using GG = Geo<D, KIND>;
+    constexpr int TG = GG::TG, UNIT = GG::UNIT, KC = GG::KC, KS = GG::KS, VC = GG::VC, VW = GG::VW, MT = GG::MT;
+    constexpr int HP = 8 * NT;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    Smem<D, NT, KIND>& sm = *reinterpret_cast<Smem<D, NT, KIND>*>(smem_raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int B = a.c.B, HS = a.c.Hk * a.HT;
+    const bool bf = KIND == BF16 || (KIND == FP8 && a.c.bf16);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    // ---- this CTA's run of units ------------------------------------------------------------
+    const int per = (B + kThreads - 1) / kThreads;
+    int mine = 0;
+    for (int b = tid * per; b < min(B, (tid + 1) * per); ++b) {
+        int lo, len;
+        seq_range(a, b, lo, len);
+        mine += seq_units<UNIT>(lo, len);
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) sm.scan[warp] = incl;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        before += w < warp ? sm.scan[w] : 0;
+        total += sm.scan[w];
+    }
+    total *= HS;
+    const int excl = before + incl - mine;
+    const int run = (total + gridDim.x - 1) / gridDim.x;
+    const int u0 = min((int64_t)run * blockIdx.x, (int64_t)total), u1 = min(u0 + run, total);
+    if (u0 < u1 && u0 >= excl * HS && u0 < (excl + mine) * HS) {
+        int b = tid * per, p = excl;
+        while (b + 1 < B) {
+            int lo, len;
+            seq_range(a, b, lo, len);
+            const int n = seq_units<UNIT>(lo, len);
+            if (u0 < (p + n) * HS) break;
+            p += n;
+            ++b;
+        }
+        sm.b = b;
+        sm.prefix = p;
+    }
+    // sequences without tokens
+    for (int b = blockIdx.x; b < B; b += gridDim.x) {
+        int lo, len;
+        seq_range(a, b, lo, len);
+        if (len > lo) continue;
+        for (int i = tid; i < a.Hq * D / 2; i += kThreads)
+            reinterpret_cast<uint32_t*>(a.out)[(int64_t)b * a.Hq * D / 2 + i] = 0;
+        if (a.lse)
+            for (int i = tid; i < a.Hq; i += kThreads) a.lse[(int64_t)b * a.Hq + i] = -INFINITY;
+        if (a.desc && a.per_stream)
+            for (int i = tid; i < HS; i += kThreads) a.desc[b * HS + i] = make_int4(0, 0, 0, 0);
+    }
+    if (a.desc && !a.per_stream && tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (u0 >= u1) return;
+    __syncthreads();
+    int b = sm.b, prefix = sm.prefix;
+
+    for (int u = u0; u < u1 && b < B;) {
+        int lo, len;
+        seq_range(a, b, lo, len);
+        const int nu = seq_units<UNIT>(lo, len);
+        if (u >= (prefix + nu) * HS) {       // past this sequence (or it is empty)
+            prefix += nu;
+            ++b;
+            continue;
+        }
+        const int rel = u - prefix * HS, stream = rel / nu, chunk = rel - stream * nu;
+        const int hk = stream / a.HT, ht = stream - hk * a.HT;
+        const int s_begin = u - chunk, s_end = s_begin + nu;       // the stream's units
+        const int chunk_end = min(nu, chunk + (u1 - u));
+        const int base = lo & ~15;
+        const int t_begin = base + chunk * UNIT, t_end = min(len, base + chunk_end * UNIT);
+        const int h0 = hk * a.G + ht * HP, nh = min(HP, a.G - ht * HP);
+        const int64_t row0 = (int64_t)b * a.Hq + h0;
+
+        // ---- queries as B fragments, in the order of the key pieces ---------------------------
+        uint32_t qf[NT][KC][KS][2];
+        float qs[NT][2];      // score factor of heads 2t, 2t + 1
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const bool have = nt * 8 + g < nh;
+            const uint16_t* qr = a.q + (row0 + nt * 8 + g) * D;
+            if (KIND != FP8) {
+#pragma unroll
+                for (int cc = 0; cc < KC; ++cc) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (have) w = ldg16(qr + (t + 4 * cc) * 8);
+                    qf[nt][cc][0][0] = w.x;
+                    qf[nt][cc][0][1] = w.y;
+                    qf[nt][cc][1][0] = w.z;
+                    qf[nt][cc][1][1] = w.w;
+                }
+                qs[nt][0] = qs[nt][1] = a.sl2;
+            } else {
+                // f16 holds a bf16 query exactly once its largest magnitude is
+                // moved to [2^14, 2^15) (what falls below 2^-24 there is 2^-38
+                // of that magnitude); the power of two goes to the score factor
+                uint4 w[KC][2];
+                uint32_t top = 0;
+#pragma unroll
+                for (int cc = 0; cc < KC; ++cc)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        w[cc][i] = make_uint4(0, 0, 0, 0);
+                        if (have) w[cc][i] = ldg16(qr + (t + 4 * cc) * 16 + 8 * i);
+                        const uint32_t ww[4] = {w[cc][i].x, w[cc][i].y, w[cc][i].z, w[cc][i].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top = max(top, max((ww[j] << 16) & 0x7FFF0000u, ww[j] & 0x7FFF0000u));
+                    }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // exponent of the largest magnitude (0 for infinities and NaN)
+                int e = top >= 0x7F800000u ? 14 : max((int)(top >> 23) - 127, -100);
+                if (!bf) e = 14;
+                const float f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+                const float back = __uint_as_float((uint32_t)(127 - 14 + e) << 23) * a.sl2;
+                qs[nt][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+                qs[nt][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+#pragma unroll
+                for (int cc = 0; cc < KC; ++cc)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t ww[4] = {w[cc][i].x, w[cc][i].y, w[cc][i].z, w[cc][i].w};
+                        if (bf) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                ww[j] = pack2<false>(__uint_as_float(ww[j] << 16) * f,
+                                                     __uint_as_float(ww[j] & 0xFFFF0000u) * f);
+                        }
+                        qf[nt][cc][2 * i][0] = ww[0];
+                        qf[nt][cc][2 * i][1] = ww[1];
+                        qf[nt][cc][2 * i + 1][0] = ww[2];
+                        qf[nt][cc][2 * i + 1][1] = ww[3];
+                    }
+            }
+        }
+
+        // ---- online softmax state ---------------------------------------------------------------
+        float o[NT][MT][4];
+        float m[NT][2], M[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+            m[nt][0] = m[nt][1] = M[nt][0] = M[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+        }
+
+        // page of the 8-token group `lane` of the tile at token t0 (-1: nothing to read)
+        const int32_t* tab = a.c.table + (int64_t)b * a.c.table_stride;
+        auto page_of = [&](int t0) {
+            const int tok = t0 + 8 * lane;
+            int pid = -1;
+            if (lane < 2 * TG && tok < t_end && tok + 7 >= lo) {
+                pid = tab[tok >> a.pshift];
+                if ((unsigned)pid >= (unsigned)a.c.n_pages) {
+                    paged_report(a.c.status, FKV_PAGED_BAD_PAGE);
+                    pid = -1;
+                }
+            }
+            return pid;
+        };
+        const int pmask = (1 << a.pshift) - 1;
+        auto line_of = [&](int pid, int tok) {
+            return (((int64_t)pid * a.c.Hk + hk) << a.pshift) + (tok & pmask);
+        };
+        uint4 kr[TG][2][KC];
+        uint32_t vr[TG][4][VC][VW];
+        float kscale[TG][2], vscale[TG][2];
+        uint32_t live = 0;      // bit 2 tg + half: row g of that 8-token group is a token to attend
+        auto load_k = [&](int t0, int pids) {
+            live = 0;
+#pragma unroll
+            for (int tg = 0; tg < TG; ++tg)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int pid = __shfl_sync(0xffffffffu, pids, 2 * tg + hf);
+                    const int tok = t0 + 16 * tg + 8 * hf + g;
+                    const bool ok = pid >= 0 && tok >= lo && tok < t_end;
+                    live |= (ok ? 1u : 0u) << (2 * tg + hf);
+                    const int64_t line = line_of(pid, tok);
+                    const unsigned char* src = reinterpret_cast<const unsigned char*>(a.c.k_pages) + line * (D * GG::ES) + 16 * t;
+#pragma unroll
+                    for (int cc = 0; cc < KC; ++cc) {
+                        kr[tg][hf][cc] = make_uint4(0, 0, 0, 0);
+                        if (ok) kr[tg][hf][cc] = ldg16(src + 64 * cc);
+                    }
+                    if (KIND == FP8) {
+                        kscale[tg][hf] = vscale[tg][hf] = 0.f;
+                        if (ok) {
+                            kscale[tg][hf] = a.c.k_scale[line];
+                            vscale[tg][hf] = a.c.v_scale[line];
+                        }
+                    }
+                }
+        };
+        auto load_v = [&](int t0, int pids) {
+#pragma unroll
+            for (int tg = 0; tg < TG; ++tg)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int pid = __shfl_sync(0xffffffffu, pids, 2 * tg + (j >> 1));
+                    const int tok = t0 + 16 * tg + 8 * (j >> 1) + 2 * t + (j & 1);
+                    const bool ok = pid >= 0 && tok >= lo && tok < t_end;
+                    const unsigned char* src = reinterpret_cast<const unsigned char*>(a.c.v_pages) +
+                                               line_of(pid, tok) * (D * GG::ES) + GG::VB * g;
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vr[tg][j][c][w] = 0;
+                        if (ok) {
+                            if (VW == 4) {
+                                const uint4 x = ldg16(src + 8 * GG::VB * c);
+                                vr[tg][j][c][0] = x.x;
+                                vr[tg][j][c][1] = x.y;
+                                vr[tg][j][c][VW - 2] = x.z;
+                                vr[tg][j][c][VW - 1] = x.w;
+                            } else {
+                                const uint2 x = ldg8(src + 8 * GG::VB * c);
+                                vr[tg][j][c][0] = x.x;
+                                vr[tg][j][c][1] = x.y;
+                            }
+                        }
+                    }
+                }
+        };
+
+        int t0 = t_begin + warp * 16 * TG;
+        int pid_cur = page_of(t0);
+        int pid_nxt = page_of(t0 + UNIT);
+        load_k(t0, pid_cur);
+        load_v(t0, pid_cur);
+        for (; t0 < t_end; t0 += UNIT) {
+            const int pid_2 = page_of(t0 + 2 * UNIT);
+            // scores
+            float x[TG][NT][4];
+#pragma unroll
+            for (int tg = 0; tg < TG; ++tg)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) x[tg][nt][0] = x[tg][nt][1] = x[tg][nt][2] = x[tg][nt][3] = 0.f;
+#pragma unroll
+            for (int tg = 0; tg < TG; ++tg)
+#pragma unroll
+                for (int cc = 0; cc < KC; ++cc) {
+                    const uint32_t r0[4] = {kr[tg][0][cc].x, kr[tg][0][cc].y, kr[tg][0][cc].z, kr[tg][0][cc].w};
+                    const uint32_t r1[4] = {kr[tg][1][cc].x, kr[tg][1][cc].y, kr[tg][1][cc].z, kr[tg][1][cc].w};
+#pragma unroll
+                    for (int st = 0; st < KS; ++st) {
+                        uint32_t a0, a1, a2, a3;
+                        if (KIND == FP8) {
+                            e4m3x4_to_h2x2(r0[st], a0, a2);
+                            e4m3x4_to_h2x2(r1[st], a1, a3);
+                        } else {
+                            a0 = r0[2 * (st & 1)];
+                            a1 = r1[2 * (st & 1)];
+                            a2 = r0[2 * (st & 1) + 1];
+                            a3 = r1[2 * (st & 1) + 1];
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma<KIND == BF16>(x[tg][nt], a0, a1, a2, a3, qf[nt][cc][st][0], qf[nt][cc][st][1]);
+                    }
+                }
+            float av[TG][2];      // log2 of the values' scales
+            float top[NT][2], topw[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = topw[nt][0] = topw[nt][1] = -INFINITY;
+#pragma unroll
+            for (int tg = 0; tg < TG; ++tg)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const bool ok = (live >> (2 * tg + hf)) & 1;
+                    if (KIND == FP8) av[tg][hf] = lg2(vscale[tg][hf]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float& s = x[tg][nt][2 * hf + i];
+                            s *= KIND == FP8 ? qs[nt][i] * kscale[tg][hf] : qs[nt][i];
+                            s = ok ? s : -INFINITY;
+                            top[nt][i] = fmaxf(top[nt][i], s);
+                            if (KIND == FP8) topw[nt][i] = fmaxf(topw[nt][i], s + av[tg][hf]);
+                        }
+                }
+            load_k(t0 + UNIT, pid_nxt);
+            // raise the running maxima when a score passes them by more than kLazy
+            bool up = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    up |= top[nt][i] > m[nt][i] + kLazy;
+                    if (KIND == FP8) up |= topw[nt][i] > M[nt][i] + kLazy;
+                }
+            if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float y = top[nt][i], z = topw[nt][i];
+#pragma unroll
+                        for (int s = 4; s < 32; s <<= 1) {
+                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, s));
+                            if (KIND == FP8) z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, s));
+                        }
+                        y = fmaxf(y, m[nt][i]);
+                        const float al = ratio2(m[nt][i], y);
+                        float aw = al;
+                        m[nt][i] = y;
+                        l[nt][i] *= al;
+                        if (KIND == FP8) {
+                            z = fmaxf(z, M[nt][i]);
+                            aw = ratio2(M[nt][i], z);
+                            M[nt][i] = z;
+                        }
+#pragma unroll
+                        for (int k = 0; k < MT; ++k) {
+                            o[nt][k][i] *= aw;
+                            o[nt][k][2 + i] *= aw;
+                        }
+                    }
+            }
+            // weights, transposed to B fragments; bf16 weights in two parts
+            // (8 bits alone would be the largest error of the product)
+            uint32_t pf[TG][NT][2], pl[TG][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+                const float M0 = M[nt][0] == -INFINITY ? 0.f : M[nt][0], M1 = M[nt][1] == -INFINITY ? 0.f : M[nt][1];
+#pragma unroll
+                for (int tg = 0; tg < TG; ++tg)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const float x0 = x[tg][nt][2 * hf], x1 = x[tg][nt][2 * hf + 1];
+                        const float p0 = ex2(x0 - m0), p1 = ex2(x1 - m1);
+                        l[nt][0] += p0;
+                        l[nt][1] += p1;
+                        float w0 = p0, w1 = p1;
+                        if (KIND == FP8) {
+                            w0 = ex2(x0 + av[tg][hf] - M0);
+                            w1 = ex2(x1 + av[tg][hf] - M1);
+                        }
+                        if (KIND == BF16) {
+                            const uint32_t hi = pack2<true>(w0, w1);
+                            const uint32_t lw = pack2<true>(w0 - __uint_as_float(hi << 16),
+                                                            w1 - __uint_as_float(hi & 0xFFFF0000u));
+                            pl[tg][nt][hf] = transpose8x8(lw);
+                            pf[tg][nt][hf] = transpose8x8(hi);
+                        } else {
+                            pf[tg][nt][hf] = transpose8x8(pack2<false>(w0, w1));
+                        }
+                    }
+            }
+            // values
+#pragma unroll
+            for (int tg = 0; tg < TG; ++tg)
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        const uint32_t* v0 = vr[tg][0][c];
+                        const uint32_t* v1 = vr[tg][1][c];
+                        const uint32_t* v2 = vr[tg][2][c];
+                        const uint32_t* v3 = vr[tg][3][c];
+                        if (KIND == FP8) {
+                            uint32_t f[2][4];      // [tokens 2t, 2t+1 | 2t+8, 2t+9][element of the word]
+                            e4m3x4_to_h2x2(prmt(v0[w], v1[w], 0x5140), f[0][0], f[0][1]);
+                            e4m3x4_to_h2x2(prmt(v0[w], v1[w], 0x7362), f[0][2], f[0][3]);
+                            e4m3x4_to_h2x2(prmt(v2[w], v3[w], 0x5140), f[1][0], f[1][1]);
+                            e4m3x4_to_h2x2(prmt(v2[w], v3[w], 0x7362), f[1][2], f[1][3]);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int i = 0; i < 2; ++i)
+                                    mma<false>(o[nt][(c * VW + w) * 2 + i], f[0][2 * i], f[0][2 * i + 1], f[1][2 * i],
+                                               f[1][2 * i + 1], pf[tg][nt][0], pf[tg][nt][1]);
+                        } else {
+                            const uint32_t a0 = prmt(v0[w], v1[w], 0x5410), a1 = prmt(v0[w], v1[w], 0x7632);
+                            const uint32_t a2 = prmt(v2[w], v3[w], 0x5410), a3 = prmt(v2[w], v3[w], 0x7632);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma<KIND == BF16>(o[nt][c * VW + w], a0, a1, a2, a3, pf[tg][nt][0], pf[tg][nt][1]);
+                                if (KIND == BF16)
+                                    mma<true>(o[nt][c * VW + w], a0, a1, a2, a3, pl[tg][nt][0], pl[tg][nt][1]);
+                            }
+                        }
+                    }
+            load_v(t0 + UNIT, pid_nxt);
+            pid_nxt = pid_2;
+        }
+
+        // ---- join the warps -----------------------------------------------------------------------
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float s = l[nt][i];
+#pragma unroll
+                for (int k = 4; k < 32; k <<= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+                if (g == 0) {
+                    sm.m[warp][nt * 8 + 2 * t + i] = m[nt][i];
+                    sm.M[warp][nt * 8 + 2 * t + i] = KIND == FP8 ? M[nt][i] : m[nt][i];
+                    sm.l[warp][nt * 8 + 2 * t + i] = s;
+                }
+#pragma unroll
+                for (int k = 0; k < MT; ++k) {
+                    // row tile k covers elements d, d + 1 of this lane's piece
+                    const int d = (k / (GG::VE / 2)) * 8 * GG::VE + g * GG::VE + 2 * (k % (GG::VE / 2));
+                    *reinterpret_cast<float2*>(&sm.o[warp][nt * 8 + 2 * t + i][d]) = make_float2(o[nt][k][i], o[nt][k][2 + i]);
+                }
+            }
+        __syncthreads();
+        const bool whole = chunk == 0 && chunk_end == nu;
+        const int slot = 2 * blockIdx.x + (u == u0 ? 0 : 1);
+        for (int i = tid; i < nh * (D / 2); i += kThreads) {
+            const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
+            float mm = -INFINITY, MM = -INFINITY, ll = 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                mm = fmaxf(mm, sm.m[w][h]);
+                MM = fmaxf(MM, sm.M[w][h]);
+            }
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                ll += sm.l[w][h] * (sm.m[w][h] == -INFINITY ? 1.f : ex2(sm.m[w][h] - mm));
+                const float f = sm.M[w][h] == -INFINITY ? 1.f : ex2(sm.M[w][h] - MM);
+                y0 += sm.o[w][h][d] * f;
+                y1 += sm.o[w][h][d + 1] * f;
+            }
+            if (whole) {
+                // all scores -inf: l = 0 and the quotient is NaN, as the formula's
+                const float f = (KIND == FP8 && MM != -INFINITY && mm != -INFINITY ? ex2(MM - mm) : 1.f) / ll;
+                y0 *= f;
+                y1 *= f;
+                const int64_t at = (row0 + h) * D + d;
+                *reinterpret_cast<uint32_t*>(a.out + at) = bf ? pack2<true>(y0, y1) : pack2<false>(y0, y1);
+                if (a.lse && d == 0) a.lse[row0 + h] = (mm + log2f(ll)) * 0.6931471805599453f;
+            } else {
+                const int64_t at = (int64_t)slot * HP + h;
+                *reinterpret_cast<float2*>(a.rec_o + at * D + d) = make_float2(y0, y1);
+                if (d == 0) a.rec_s[at] = make_float4(mm, MM, ll, 0.f);
+            }
+        }
+        if (a.desc && chunk == 0 && tid == 0) {
+            // the CTA that holds a stream's first unit says how to join it
+            int pieces = whole ? 0 : (s_end - 1) / run - (int)blockIdx.x + 1;
+            const int4 d = make_int4((int)row0, nh, pieces, slot);
+            if (a.per_stream) a.desc[b * HS + stream] = d;
+            else if (!whole) a.desc[blockIdx.x] = d;
+        }
+        u += chunk_end - chunk;
+        __syncthreads();
+    }
+}
+
+constexpr int kJoinThreads = 128;
+
+// Joins the pieces of one split stream for one head: piece 0 is record
+// `first`, piece j > 0 the first record of the j-th CTA after it.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttendArgs a, int HP, bool fp8) {
+    constexpr int LPR = D / 4 < 32 ? D / 4 : 32;            // lanes of one record's row
+    constexpr int V4 = D / (4 * LPR), GROUPS = kJoinThreads / LPR;
+    __shared__ float so[GROUPS][D];
+    __shared__ float ss[GROUPS][3];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 ds = a.desc[blockIdx.x];
+    const int h = blockIdx.y;
+    if (ds.z == 0 || h >= ds.y) return;
+    const int grp = threadIdx.x / LPR, ln = threadIdx.x % LPR;
+    const int cta = ds.w >> 1;
+    float m = -INFINITY, M = -INFINITY, l = 0.f;
+    float4 o[V4];
+#pragma unroll
+    for (int v = 0; v < V4; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int j = grp; j < ds.z; j += GROUPS) {
+        const int64_t at = (int64_t)(j == 0 ? ds.w : 2 * (cta + j)) * HP + h;
+        const float4 s = a.rec_s[at];
+        float4 x[V4];
+#pragma unroll
+        for (int v = 0; v < V4; ++v) x[v] = *reinterpret_cast<const float4*>(a.rec_o + at * D + 4 * (ln + v * LPR));
+        const float mn = fmaxf(m, s.x), Mn = fmaxf(M, s.y);
+        const float fa = m == -INFINITY ? 1.f : ex2(m - mn), fb = s.x == -INFINITY ? 1.f : ex2(s.x - mn);
+        const float ga = M == -INFINITY ? 1.f : ex2(M - Mn), gb = s.y == -INFINITY ? 1.f : ex2(s.y - Mn);
+        l = l * fa + s.z * fb;
+#pragma unroll
+        for (int v = 0; v < V4; ++v) {
+            o[v].x = o[v].x * ga + x[v].x * gb;
+            o[v].y = o[v].y * ga + x[v].y * gb;
+            o[v].z = o[v].z * ga + x[v].z * gb;
+            o[v].w = o[v].w * ga + x[v].w * gb;
+        }
+        m = mn;
+        M = Mn;
+    }
+#pragma unroll
+    for (int v = 0; v < V4; ++v) *reinterpret_cast<float4*>(&so[grp][4 * (ln + v * LPR)]) = o[v];
+    if (ln == 0) {
+        ss[grp][0] = m;
+        ss[grp][1] = M;
+        ss[grp][2] = l;
+    }
+    __syncthreads();
+    float mm = -INFINITY, MM = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < GROUPS; ++w) {
+        mm = fmaxf(mm, ss[w][0]);
+        MM = fmaxf(MM, ss[w][1]);
+    }
+#pragma unroll
+    for (int w = 0; w < GROUPS; ++w) ll += ss[w][2] * (ss[w][0] == -INFINITY ? 1.f : ex2(ss[w][0] - mm));
+    const float f = (fp8 && MM != -INFINITY && mm != -INFINITY ? ex2(MM - mm) : 1.f) / ll;
+    for (int d = threadIdx.x * 2; d < D; d += kJoinThreads * 2) {
+        float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < GROUPS; ++w) {
+            const float x = ss[w][1] == -INFINITY ? 1.f : ex2(ss[w][1] - MM);
+            y0 += so[w][d] * x;
+            y1 += so[w][d + 1] * x;
+        }
+        const int64_t at = (int64_t)(ds.x + h) * D + d;
+        *reinterpret_cast<uint32_t*>(a.out + at) = a.c.bf16 ? pack2<true>(y0 * f, y1 * f) : pack2<false>(y0 * f, y1 * f);
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[ds.x + h] = (mm + log2f(ll)) * 0.6931471805599453f;
+}
+
+struct Plan {
+    int nt, ht, unit, ctas, streams;
+    bool split, per_stream;
+    size_t bytes, off_s, off_d;
+};
+
+using Kernel = void (*)(const AttendArgs);
+
+template <int D, int NT, int KIND>
+void entry(Kernel& k, size_t& smem) {
+    k = attend_kernel<D, NT, KIND>;
+    smem = sizeof(Smem<D, NT, KIND>);
+}
+
+template <int D>
+void entry_d(int nt, int kind, Kernel& k, size_t& smem) {
+    if constexpr (D == 256) {           // 16 heads' accumulators do not fit the registers
+        switch (kind) {
+            case F16: entry<D, 1, F16>(k, smem); break;
+            case BF16: entry<D, 1, BF16>(k, smem); break;
+            default: entry<D, 1, FP8>(k, smem); break;
+        }
+    } else switch (nt * 4 + kind) {
+        case 4: entry<D, 1, F16>(k, smem); break;
+        case 5: entry<D, 1, BF16>(k, smem); break;
+        case 6: entry<D, 1, FP8>(k, smem); break;
+        case 8: entry<D, 2, F16>(k, smem); break;
+        case 9: entry<D, 2, BF16>(k, smem); break;
+        default: entry<D, 2, FP8>(k, smem); break;
+    }
+}
+
+int kind_of(const FkvPagedCache* c) { return c->fp8 ? FP8 : c->bf16 ? BF16 : F16; }
+
+// CTAs of one wave of a kernel on the current device; the kernel's shared
+// memory limit is raised on its first use on that device.
+int wave(Kernel k, size_t smem, int dev, int* out) {
+    static std::mutex mu;
+    static struct { Kernel k; int dev, n; } memo[256];
+    static int used = 0;
+    std::lock_guard<std::mutex> lock(mu);
+    for (int i = 0; i < used; ++i)
+        if (memo[i].k == k && memo[i].dev == dev) {
+            *out = memo[i].n;
+            return FKV_OK;
+        }
+    FKV_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    int per_sm = 0, sms = 0;
+    FKV_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kThreads, smem));
+    FKV_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    FKV_REQUIRE(per_sm > 0 && sms > 0, FKV_ERR_CUDA, "fkv_paged_attend: kernel does not fit an SM");
+    *out = per_sm * sms;
+    if (used < 256) memo[used++] = {k, dev, *out};
+    return FKV_OK;
+}
+
+constexpr int kMaxCtas = 148 * 3;     // bound of any wave here, for sizing without a device
+
+// 8-head tiles that one warp takes together
+int tiles_of(int G, int D) { return G <= 8 || D == 256 ? 1 : 2; }
+
+int make_plan(const FkvPagedCache* c, int Hq, int pshift, int ctas, Plan* p) {
+    const int G = Hq / c->Hk;
+    p->nt = tiles_of(G, c->D);
+    p->ht = (G + 8 * p->nt - 1) / (8 * p->nt);
+    const int es = c->fp8 ? 1 : 2;
+    p->unit = kWarps * 16 * (c->D * es >= 256 ? 1 : 2);
+    const int64_t reach = (int64_t)c->width << pshift;
+    const int64_t units = (reach + 15 + p->unit - 1) / p->unit;
+    const int64_t streams = (int64_t)c->B * c->Hk * p->ht;
+    FKV_REQUIRE(streams * std::max<int64_t>(units, 1) < INT_MAX / 2 && (int64_t)c->B * Hq < INT_MAX,
+                FKV_ERR_UNSUPPORTED, "fkv_paged_attend: %lld streams of %lld tokens are too many",
+                (long long)streams, (long long)reach);
+    p->streams = (int)streams;
+    const int64_t most = std::max<int64_t>(1, streams * std::max<int64_t>(units, 1));
+    p->ctas = (int)std::min<int64_t>(ctas, most);
+    p->split = units > 1;
+    p->per_stream = p->streams <= p->ctas;
+    const int hp = 8 * p->nt;
+    const size_t recs = 2 * (size_t)p->ctas * hp;
+    p->off_s = recs * c->D * sizeof(float);
+    p->off_d = p->off_s + recs * sizeof(float4);
+    p->bytes = p->split ? p->off_d + (size_t)std::max(p->ctas, 1) * sizeof(int4) : 0;
+    return FKV_OK;
+}
+
+}  // namespace
+
+extern "C" size_t fkv_paged_attend_workspace_bytes(const FkvPagedCache* c, int32_t Hq) {
+    int pshift = 0;
+    Plan p;
+    FkvPagedCache s;
+    if (c == nullptr) return 0;
+    s = *c;
+    if (s.D != 64 && s.D != 128 && s.D != 256) return 0;
+    if (s.page < 8 || s.page > 256 || (s.page & (s.page - 1)) || s.Hk < 1 || s.B < 0 || s.width < 0) return 0;
+    while ((1 << pshift) < s.page) ++pshift;
+    if (Hq < 1 || Hq % s.Hk != 0 || ((int64_t)s.width << pshift) > INT_MAX) return 0;
+    return make_plan(&s, Hq, pshift, kMaxCtas, &p) == FKV_OK ? p.bytes : 0;
+}
+
+extern "C" int fkv_paged_attend(const FkvPagedCache* c, int32_t Hq, float scale, int32_t window,
+                                const uint16_t* q, uint16_t* out, float* lse, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+    int pshift = 0;
+    int rc = fkv::paged_check(c, "fkv_paged_attend", &pshift);
+    if (rc != FKV_OK) return rc;
+    FKV_REQUIRE(Hq >= 1 && Hq % c->Hk == 0, FKV_ERR_INVALID,
+                "fkv_paged_attend: Hq=%d is not a multiple of Hk=%d", Hq, c->Hk);
+    FKV_REQUIRE(window >= 0, FKV_ERR_INVALID, "fkv_paged_attend: window %d", window);
+    if (c->B == 0) return FKV_OK;
+    FKV_REQUIRE(q && out, FKV_ERR_INVALID, "fkv_paged_attend: NULL pointer");
+    FKV_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0, FKV_ERR_INVALID,
+                "fkv_paged_attend: q / out not 16-byte aligned");
+    const int G = Hq / c->Hk, nt = tiles_of(G, c->D);
+    Kernel k;
+    size_t smem;
+    if (c->D == 64) entry_d<64>(nt, kind_of(c), k, smem);
+    else if (c->D == 128) entry_d<128>(nt, kind_of(c), k, smem);
+    else entry_d<256>(nt, kind_of(c), k, smem);
+    int dev = 0, ctas = 0;
+    Plan p;
+    rc = make_plan(c, Hq, pshift, kMaxCtas, &p);
+    if (rc != FKV_OK) return rc;
+    FKV_CUDA_CHECK(cudaGetDevice(&dev));
+    rc = wave(k, smem, dev, &ctas);
+    if (rc != FKV_OK) return rc;
+    rc = make_plan(c, Hq, pshift, std::min(ctas, kMaxCtas), &p);
+    if (rc != FKV_OK) return rc;
+    FKV_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes), FKV_ERR_INVALID,
+                "fkv_paged_attend: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
+    FKV_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, FKV_ERR_INVALID,
+                "fkv_paged_attend: workspace not 16-byte aligned");
+    AttendArgs a;
+    a.c = *c;
+    a.q = q;
+    a.out = out;
+    a.lse = lse;
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    a.rec_o = p.split ? reinterpret_cast<float*>(ws) : nullptr;
+    a.rec_s = p.split ? reinterpret_cast<float4*>(ws + p.off_s) : nullptr;
+    a.desc = p.split ? reinterpret_cast<int4*>(ws + p.off_d) : nullptr;
+    a.Hq = Hq;
+    a.G = G;
+    a.HT = p.ht;
+    a.pshift = pshift;
+    a.window = window;
+    a.per_stream = p.per_stream;
+    a.sl2 = scale * 1.4426950408889634f;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    k<<<p.ctas, kThreads, smem, s>>>(a);
+    FKV_LAUNCH_CHECK();
+    if (!p.split) return FKV_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.per_stream ? p.streams : p.ctas, std::min(G, 8 * nt));
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const bool fp8 = c->fp8 != 0;
+    if (c->D == 64) FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<64>, a, 8 * nt, fp8));
+    else if (c->D == 128) FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<128>, a, 8 * nt, fp8));
+    else FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<256>, a, 8 * nt, fp8));
+    return FKV_OK;
+}

@@ -1,0 +1,363 @@
+"""Paged key-value cache: sequences of any lengths in one pool of pages, next
+to the tiered cache, which wants one length for a whole batch (no counterpart
+in the reference).
+
+``paged_append`` writes new tokens (rotating and quantising them on the way),
+``paged_attend`` attends one new token per sequence over its pages, and
+``paged_read`` gives a sequence back as dense keys and values, for instance
+for ``compress_layer``.  ``PagedKVCache`` keeps the pages, the page table and
+the free list of all layers.
+
+Tensors shared by the three functions, P pages of ``page`` tokens:
+  k_pages, v_pages  (P, Hk, page, D) float16, bfloat16 or float8_e4m3fn; D 64,
+                    128 or 256, page a power of two from 8 to 256
+  k_scale, v_scale  (P, Hk, page) float32, for float8 pages: a stored row is
+                    its codes times this
+  table             (B, W) int32: page of tokens [j * page, (j + 1) * page) of
+                    sequence b; entries behind a sequence's end are not read
+  lens              (B,) int32: tokens of each sequence, new ones included
+  status            optional int32 word of sticky error bits: 1 = a table entry
+                    that is no page (its tokens are left out), 2 = a length or
+                    position outside the table
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence
+
+import torch
+
+from . import _native
+from .cache import FoveatedKVCache, compress_layer
+from .config import TierConfig
+from .rotary import check_frequencies, on_device, refuse_grad, rows16
+
+_F16 = torch.float16
+_BF16 = torch.bfloat16
+_F8 = torch.float8_e4m3fn
+_I32 = torch.int32
+BAD_PAGE, BAD_POSITION = 1, 2
+
+
+def _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dtype):
+    """The checked descriptor of the pages; dtype is that of the tensors beside them."""
+    dev, kind = k_pages.device, k_pages.dtype
+    if not k_pages.is_cuda:
+        raise ValueError(f"{who}: pages must be CUDA tensors")
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype is not kind or v_pages.device != dev \
+            or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+        raise ValueError(f"{who}: k_pages and v_pages must be contiguous (P, Hk, page, D) of one type and device")
+    if dtype is not _F16 and dtype is not _BF16:
+        raise ValueError(f"{who}: {dtype} beside the pages, expected float16 or bfloat16")
+    fp8 = kind is _F8
+    if not fp8 and kind is not dtype:
+        raise ValueError(f"{who}: pages of {kind} beside {dtype}, expected the same type or float8_e4m3fn pages")
+    P, Hk, page, D = k_pages.shape
+    if fp8:
+        for s in (k_scale, v_scale):
+            if s is None or s.dtype is not torch.float32 or s.device != dev or s.shape != (P, Hk, page) \
+                    or not s.is_contiguous():
+                raise ValueError(f"{who}: float8 pages need contiguous float32 k_scale and v_scale (P, Hk, page)")
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError(f"{who}: scales go with float8 pages only")
+    if table.dtype is not _I32 or table.dim() != 2 or table.device != dev or lens.dtype is not _I32 \
+            or lens.device != dev or lens.shape != table.shape[:1] or not lens.is_contiguous():
+        raise ValueError(f"{who}: table must be int32 (B, W) and lens contiguous int32 (B,) on {dev}")
+    B, W = table.shape
+    stride = table.stride(0) if B > 1 else W
+    if (W > 1 and table.stride(1) != 1) or stride < W:
+        raise ValueError(f"{who}: a row of table must be contiguous, and rows must not overlap")
+    if status is not None and (status.dtype is not _I32 or status.device != dev or status.numel() != 1):
+        raise ValueError(f"{who}: status must be one int32 on {dev}")
+    return _native.PagedCache(
+        k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr() if fp8 else None,
+        v_scale.data_ptr() if fp8 else None, table.data_ptr(), lens.data_ptr(),
+        None if status is None else status.data_ptr(), B, Hk, D, page, P, W, stride, fp8, dtype is _BF16)
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 table: torch.Tensor, lens: torch.Tensor, *, cu_new: Optional[torch.Tensor] = None,
+                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                 q: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
+                 interleaved: bool = False, amplitude: float = 1.0, q_out: Optional[torch.Tensor] = None,
+                 status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Write new tokens into their sequences' pages, in one launch.
+
+    k, v (B, Hk, n, D): n tokens for each sequence; or (B, Hk, D): one token
+    each; a sequence of length 0 is an empty slot and gets none.  With cu_new
+    (B + 1,) int32: packed rows (T, Hk, D), sequence b's are
+    [cu_new[b], cu_new[b + 1]), rows behind the last are padding.  The new
+    tokens are the last of their sequences (``lens`` counts them), and two
+    sequences must not be given the same page to write.
+
+    With inv_freq the keys are rotated by their positions before they are
+    stored (``apply_rotary``'s arguments), and so is q, which has k's layout
+    and Hq heads; the rotated q is returned (q_out, which may be q itself, or a
+    new tensor), zeros for tokens that are not stored.  float8 pages quantise
+    each row: scale = max(|row|, 2^-100) / 448, a row with an infinity or a NaN
+    reads back as NaN.
+    """
+    who = "paged_append"
+    dt, dev, nd = k.dtype, k_pages.device, k.dim()
+    refuse_grad(who, k, v, q)
+    c = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dt)
+    if v.shape != k.shape or nd not in (3, 4) or (nd == 4 and cu_new is not None) \
+            or k.shape[1] != c.Hk or k.shape[-1] != c.D:
+        raise ValueError(f"{who}: k {tuple(k.shape)} and v {tuple(v.shape)} must be (tokens, {c.Hk}, {c.D}), "
+                         f"or (B, {c.Hk}, n, {c.D}) without cu_new")
+    n = _native.PagedNew()
+    T = k.shape[0]
+    if cu_new is not None:
+        if cu_new.dtype is not _I32 or cu_new.device != dev or cu_new.shape != (c.B + 1,) or not cu_new.is_contiguous():
+            raise ValueError(f"{who}: cu_new must be contiguous int32 (B + 1,) on {dev}")
+        n.cu_new = cu_new.data_ptr()
+    else:
+        if T != c.B:
+            raise ValueError(f"{who}: k holds {T} sequences, the table {c.B}")
+        n.n_uniform = k.shape[2] if nd == 4 else 1
+        T *= n.n_uniform
+    n.T = T
+    if (q is None) != (inv_freq is None) and inv_freq is None:
+        raise ValueError(f"{who}: q is only rotated; pass inv_freq with it")
+    if inv_freq is not None:
+        check_frequencies(who, inv_freq, dev)
+        n.rot, n.inv_freq = 2 * inv_freq.numel(), inv_freq.data_ptr()
+        n.interleaved, n.amplitude = interleaved, amplitude
+    rows = [("k", k, n.k_stride), ("v", v, n.v_stride)]
+    if q is not None:
+        if q.dim() != nd or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+            raise ValueError(f"{who}: q {tuple(q.shape)} does not go with k {tuple(k.shape)}")
+        n.Hq = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=dt, device=dev)
+        elif q_out.shape != q.shape or rows16(who, "q_out", q_out, dt, dev) is not q_out \
+                or any(m > 1 and s == 0 for m, s in zip(q_out.shape, q_out.stride())):
+            raise ValueError(f"{who}: q_out has another shape, or is not 8-byte aligned rows with strides of a "
+                             "multiple of 4 elements")
+        rows += [("q", q, n.q_stride), ("q_out", q_out, n.q_out_stride)]
+    elif q_out is not None:
+        raise ValueError(f"{who}: q_out without q")
+    keep = []
+    for name, t, f in rows:
+        t = rows16(who, name, t, dt, dev)
+        st = t.stride()
+        f[:] = (st[0], st[2], st[1]) if nd == 4 else (st[0], 0 if cu_new is None else st[0], st[1])
+        setattr(n, name, t.data_ptr())
+        keep.append(t)
+    _native.check(on_device(dev, _native.load().fkv_paged_append, C.byref(c), C.byref(n)), "fkv_paged_append")
+    return q_out
+
+
+def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, max_len: int,
+               *, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+               dtype: Optional[torch.dtype] = None, status: Optional[torch.Tensor] = None):
+    """The sequences' first max_len tokens as dense (k, v), each
+    (B, Hk, max_len, D) of ``dtype`` (the pages' own type, or float16 for
+    float8 pages), with zeros behind a sequence's end."""
+    who = "paged_read"
+    if dtype is None:
+        dtype = _F16 if k_pages.dtype is _F8 else k_pages.dtype
+    c = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dtype)
+    if max_len < 0:
+        raise ValueError(f"{who}: max_len {max_len}")
+    k = torch.empty((c.B, c.Hk, max_len, c.D), dtype=dtype, device=k_pages.device)
+    v = torch.empty_like(k)
+    _native.check(on_device(k_pages.device, _native.load().fkv_paged_read, C.byref(c), max_len, k.data_ptr(),
+                            v.data_ptr()), "fkv_paged_read")
+    return k, v
+
+
+def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                 lens: torch.Tensor, *, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None, scale: Optional[float] = None, window: int = 0,
+                 return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                 status: Optional[torch.Tensor] = None):
+    """Attention of one new token per sequence over its pages.
+
+    q (B, Hq, D) or (B, Hq, 1, D), Hq a multiple of Hk; ``scale`` 1/sqrt(D) by
+    default; ``window`` > 0 attends the last ``window`` tokens only.  Returns
+    out, of q's shape, and with return_lse the natural log-sum-exp of the
+    scaled scores, (B, Hq) float32.  A sequence without tokens gives zeros and
+    -inf.  Lengths are read on the device, so the call can be captured once and
+    replayed as sequences grow within the table.
+    """
+    who = "paged_attend"
+    dt, dev = q.dtype, k_pages.device
+    refuse_grad(who, q)
+    c = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dt)
+    shape = q.shape
+    if q.device != dev or len(shape) not in (3, 4) or shape[0] != c.B or shape[-1] != c.D \
+            or (len(shape) == 4 and shape[2] != 1) or shape[1] < 1 or shape[1] % c.Hk:
+        raise ValueError(f"{who}: q {tuple(shape)} must be (B, Hq, D) or (B, Hq, 1, D) on {dev} with B {c.B}, "
+                         f"D {c.D} and Hq a multiple of {c.Hk}")
+    if window < 0:
+        raise ValueError(f"{who}: window {window}")
+    Hq = shape[1]
+    if not q.is_contiguous():
+        q = q.contiguous()
+    if q.data_ptr() & 15:
+        q = q.clone()
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=dev)
+    elif out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous() \
+            or out.data_ptr() & 15:
+        raise ValueError(f"{who}: out must be a contiguous, 16-byte aligned tensor like q")
+    lse = torch.empty((c.B, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    lib = _native.load()
+    nbytes = lib.fkv_paged_attend_workspace_bytes(C.byref(c), Hq)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _native.check(on_device(dev, lib.fkv_paged_attend, C.byref(c), Hq, c.D ** -0.5 if scale is None else scale,
+                            window, q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+                            None if ws is None else ws.data_ptr(), nbytes), "fkv_paged_attend")
+    return (out, lse) if return_lse else out
+
+
+class PagedKVCache:
+    """Pages, page table and free list of all layers of a serving batch.
+
+    A slot (row of the batch) holds one sequence.  A step is ``extend(counts)``
+    (pages for the new tokens, lengths and table on the device), then for every
+    layer ``append`` and ``attend``; ``release(slot)`` gives its pages back.
+    With at most one new token per slot, k, v and q of the step have a row per
+    slot (rows of slots without a new token are ignored); otherwise they are
+    packed, in slot order.  ``append`` and ``attend`` can be captured in a CUDA
+    graph between ``extend`` calls of the same kind: the page table, lengths and
+    counts they read are updated in place.
+    """
+
+    def __init__(self, n_layers: int, n_pages: int, H_kv: int, D: int, *, page: int = 16, max_seqs: int = 1,
+                 max_len: int, fmt: str = "16", dtype: torch.dtype = _F16, inv_freq=None, interleaved: bool = False,
+                 amplitude: float = 1.0, device="cuda"):
+        if fmt not in ("16", "fp8"):
+            raise ValueError(f"fmt must be '16' or 'fp8', got {fmt!r}")
+        if dtype not in (_F16, _BF16):
+            raise ValueError(f"dtype must be float16 or bfloat16, got {dtype}")
+        if min(n_layers, n_pages, H_kv, max_seqs, max_len) < 1:
+            raise ValueError("sizes must be at least 1")
+        if D not in (64, 128, 256):
+            raise ValueError(f"head dim {D} unsupported (64, 128 or 256)")
+        if page < 8 or page > 256 or page & (page - 1):
+            raise ValueError(f"page {page} is not a power of two from 8 to 256")
+        self.n_layers, self.n_pages, self.H_kv, self.D = n_layers, n_pages, H_kv, D
+        self.page, self.max_seqs, self.max_len, self.dtype, self.fmt = page, max_seqs, max_len, dtype, fmt
+        self.inv_freq, self.interleaved, self.amplitude = inv_freq, interleaved, float(amplitude)
+        shape = (n_pages, H_kv, page, D)
+        kind = _F8 if fmt == "fp8" else dtype
+        new = lambda: torch.zeros(shape, dtype=torch.uint8 if kind is _F8 else kind, device=device).view(kind)
+        scale = lambda: torch.zeros(shape[:3], dtype=torch.float32, device=device) if kind is _F8 else None
+        self.layers = [dict(k_pages=new(), v_pages=new(), k_scale=scale(), v_scale=scale()) for _ in range(n_layers)]
+        self.width = -(-max_len // page)
+        self.table = torch.full((max_seqs, self.width), -1, dtype=_I32, device=device)
+        self.lens = torch.zeros(max_seqs, dtype=_I32, device=device)
+        self.status = torch.zeros(1, dtype=_I32, device=device)
+        self.device = self.table.device
+        self._step_lens = torch.zeros(max_seqs, dtype=_I32, device=device)   # 0: no new token in this step
+        self._cu = torch.zeros(max_seqs + 1, dtype=_I32, device=device)
+        self._packed = None                                                   # None: no step begun
+        self._new_rows = 0
+        self._lens = [0] * max_seqs
+        self._pages = [[] for _ in range(max_seqs)]
+        self._free = list(range(n_pages - 1, -1, -1))
+
+    @property
+    def lengths(self) -> list:
+        return list(self._lens)
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def extend(self, counts: Sequence[int]) -> None:
+        """Begin a step that adds counts[slot] tokens to each slot: takes pages
+        and updates the table and the lengths.  Nothing changes when the pages
+        do not suffice or a sequence would pass max_len."""
+        counts = [int(c) for c in counts]
+        if len(counts) != self.max_seqs or min(counts) < 0:
+            raise ValueError(f"extend: need {self.max_seqs} counts of 0 or more")
+        lens = [a + c for a, c in zip(self._lens, counts)]
+        if max(lens) > self.max_len:
+            raise ValueError(f"extend: a sequence of {max(lens)} tokens passes max_len {self.max_len}")
+        need = [-(-n // self.page) - len(p) for n, p in zip(lens, self._pages)]
+        if sum(need) > len(self._free):
+            raise _native.FkvNativeError(f"extend: {sum(need)} pages needed, {len(self._free)} free")
+        at, ids = [], []
+        for s, m in enumerate(need):
+            for _ in range(m):
+                at.append(s * self.width + len(self._pages[s]))
+                ids.append(self._free.pop())
+                self._pages[s].append(ids[-1])
+        if at:
+            upd = torch.tensor([at, ids], dtype=torch.int64).to(self.device)
+            self.table.view(-1)[upd[0]] = upd[1].to(_I32)
+        self._lens = lens
+        self._packed = max(counts) > 1
+        self._new_rows = sum(counts) if self._packed else self.max_seqs
+        cu = [0]
+        for c in counts:
+            cu.append(cu[-1] + c)
+        host = torch.tensor(lens + [n if c else 0 for n, c in zip(lens, counts)] + cu, dtype=_I32).to(self.device)
+        n = self.max_seqs
+        self.lens.copy_(host[:n])
+        self._step_lens.copy_(host[n:2 * n])
+        self._cu.copy_(host[2 * n:])
+
+    def release(self, slot: int) -> None:
+        """Empty a slot; its pages may be given to other sequences."""
+        self._free.extend(reversed(self._pages[slot]))
+        self._pages[slot] = []
+        self._lens[slot] = 0
+        self.table[slot].fill_(-1)
+        self.lens[slot:slot + 1].zero_()
+        self._step_lens[slot:slot + 1].zero_()
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, q: Optional[torch.Tensor] = None):
+        """Write the step's keys and values of one layer; returns q, rotated
+        if the cache has rotary frequencies (keys are then stored rotated)."""
+        if self._packed is None:
+            raise ValueError("append: call extend first")
+        if k.shape[0] != self._new_rows if not self._packed else k.shape[0] < self._new_rows:
+            raise ValueError(f"append: {k.shape[0]} rows of k, the step has {self._new_rows}")
+        turn = {} if self.inv_freq is None else dict(inv_freq=self.inv_freq, interleaved=self.interleaved,
+                                                     amplitude=self.amplitude, q=q)
+        lens, cu = (self.lens, self._cu) if self._packed else (self._step_lens, None)
+        r = paged_append(k, v, table=self.table, lens=lens, cu_new=cu, status=self.status, **turn,
+                         **self.layers[layer])
+        return q if self.inv_freq is None else r
+
+    def attend(self, layer: int, q: torch.Tensor, *, scale: Optional[float] = None, window: int = 0,
+               return_lse: bool = False, out: Optional[torch.Tensor] = None):
+        """Attention of one token per slot, q (max_seqs, Hq, D), over its sequence."""
+        return paged_attend(q, table=self.table, lens=self.lens, scale=scale, window=window, return_lse=return_lse,
+                            out=out, status=self.status, **self.layers[layer])
+
+    def read(self, layer: int, slot: int):
+        """One sequence as dense keys and values (1, H_kv, length, D)."""
+        n = self._lens[slot]
+        return paged_read(table=self.table[slot:slot + 1], lens=self.lens[slot:slot + 1], max_len=n,
+                          dtype=self.dtype, status=self.status, **self.layers[layer])
+
+    def compress(self, slot: int, cfg: Optional[TierConfig] = None, query=None,
+                 keep_archive: bool = True) -> FoveatedKVCache:
+        """Hand one sequence to the tiered cache: every layer read back and
+        tiered by ``compress_layer``.  The slot keeps its pages."""
+        fov = FoveatedKVCache(cfg)
+        fov.layers = [compress_layer(*self.read(i, slot), fov.cfg,
+                                     query[i] if isinstance(query, (list, tuple)) else query, keep_archive)
+                      for i in range(self.n_layers)]
+        fov.seq_length = self._lens[slot]
+        fov._compressed = True
+        return fov
+
+    def check(self) -> None:
+        """Raise FkvNativeError if a launch met a bad page or position since
+        the last check.  Waits for the current stream."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            what = [t for b, t in ((BAD_PAGE, "a table entry that is no page"),
+                                   (BAD_POSITION, "a length or position outside the table")) if bits & b]
+            raise _native.FkvNativeError("paged cache: " + " and ".join(what))
+
+    def memory_bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for lay in self.layers for t in lay.values() if t is not None)

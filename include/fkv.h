@@ -311,6 +311,99 @@ int fkv_ipc_open(const uint8_t* handle, int64_t offset, void** dev_ptr);
 int fkv_ipc_close(void* dev_ptr, int64_t offset);
 
 /* ------------------------------------------------------------------------ */
+/* Rotary positions                                                         */
+/* ------------------------------------------------------------------------ */
+
+/* Sizes and strides of fkv_rotary.  Tensors are 16-bit (fp16, or bf16 when
+ * bf16 != 0), token (b, s) of head h at b * stride[0] + s * stride[1] +
+ * h * stride[2] elements; elements of a head are contiguous. */
+typedef struct FkvRotaryShape {
+    int32_t B, S, Hq, Hk, D;   /* Hq or Hk may be 0 */
+    int32_t rot;               /* rotated elements of a head: a multiple of 8, <= D */
+    int32_t bf16;
+    int32_t interleaved;       /* pairs (2p, 2p + 1); otherwise (p, p + rot / 2) */
+    int32_t inverse;           /* turn back */
+    int32_t pos64;             /* positions are int64; otherwise int32 */
+    float amplitude;           /* factor of the rotated part */
+    int32_t reserved;
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];
+    int64_t pos_stride[2];
+} FkvRotaryShape;
+
+/* q and k turned by their tokens' positions, in one launch (no counterpart in
+ * the reference).  inv_freq: rot / 2 doubles on the device, radians per
+ * position; angles are reduced to one turn in 64 bits.  q_out / k_out may be
+ * q / k themselves.  Pointers 8-byte aligned, strides multiples of 4. */
+int fkv_rotary(const FkvRotaryShape* s, const uint16_t* q, const uint16_t* k,
+               const void* positions, const double* inv_freq, uint16_t* q_out, uint16_t* k_out,
+               void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Paged key-value cache                                                    */
+/* ------------------------------------------------------------------------ */
+
+/* One layer's pages, and the sequences in them (no counterpart in the
+ * reference, whose cache holds whole sequences of one length). */
+typedef struct FkvPagedCache {
+    void *k_pages, *v_pages;     /* (n_pages, Hk, page, D): fp16 / bf16, or E4M3 codes if fp8 */
+    float *k_scale, *v_scale;    /* (n_pages, Hk, page): factor of a row's codes (fp8 only) */
+    const int32_t* table;        /* (B, width): page of tokens [j * page, (j + 1) * page) */
+    const int32_t* lens;         /* (B): tokens of a sequence, new ones included */
+    int32_t* status;             /* sticky FKV_PAGED_* bits, zero-filled once; may be NULL */
+    int32_t B, Hk, D;            /* D: 64, 128 or 256 */
+    int32_t page;                /* tokens of a page: a power of two from 8 to 256 */
+    int32_t n_pages;
+    int32_t width;               /* table entries of a sequence */
+    int32_t table_stride;        /* entries from one sequence's row to the next, >= width */
+    int32_t fp8;
+    int32_t bf16;                /* type of 16-bit pages and of every tensor beside them */
+    int32_t reserved;
+} FkvPagedCache;
+
+#define FKV_PAGED_BAD_PAGE 1     /* a table entry that is no page: its tokens are left out */
+#define FKV_PAGED_BAD_POSITION 2 /* a length or position outside the table's reach */
+
+/* New tokens, (token, head) rows with any strides (multiples of 4 elements,
+ * pointers 8-byte aligned).  cu_new == NULL: n_uniform tokens for each of the
+ * B sequences, token (b, i) at b * stride[0] + i * stride[1]; a sequence of
+ * length 0 is an empty slot and gets none.  Otherwise sequence b's are tokens
+ * [cu_new[b], cu_new[b + 1]) at t * stride[1], and tokens behind cu_new[B]
+ * are padding.  They are the last tokens of their sequences. */
+typedef struct FkvPagedNew {
+    const uint16_t *k, *v;       /* (T, Hk, D) */
+    const uint16_t* q;           /* (T, Hq, D), NULL if Hq == 0 */
+    uint16_t* q_out;             /* rotated queries; zeros for tokens that are not stored */
+    const int32_t* cu_new;
+    const double* inv_freq;      /* rot / 2, as fkv_rotary */
+    int64_t k_stride[3], v_stride[3], q_stride[3], q_out_stride[3];
+    int32_t T, n_uniform, Hq;
+    int32_t rot;                 /* 0: keys are stored as they come */
+    int32_t interleaved;
+    float amplitude;
+} FkvPagedNew;
+
+/* Writes the new tokens' keys (rotated by their positions) and values into
+ * their pages and rotates their queries, in one launch.  fp8: scale =
+ * max(|row|, 2^-100) / 448, code = e4m3(x * (448 / max)) to nearest even; a
+ * row with a NaN or an infinity reads back as NaN.  Two tokens must not share
+ * a place: a page that is being written belongs to one sequence. */
+int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, void* stream);
+
+/* The sequences as dense (B, Hk, max_len, D) 16-bit keys and values, zeros
+ * behind a sequence's end. */
+int fkv_paged_read(const FkvPagedCache* c, int32_t max_len, uint16_t* k, uint16_t* v, void* stream);
+
+/* Attention of one token per sequence over its last `window` tokens (0: all):
+ * q, out (B, Hq, D) 16-bit, 16-byte aligned; lse (B, Hq) f32 natural
+ * log-sum-exp of the scaled scores, or NULL.  A sequence without tokens gives
+ * zeros and -inf.  The workspace needs no initialisation; calls that share
+ * one must not overlap on the GPU. */
+size_t fkv_paged_attend_workspace_bytes(const FkvPagedCache* c, int32_t Hq);
+int fkv_paged_attend(const FkvPagedCache* c, int32_t Hq, float scale, int32_t window,
+                     const uint16_t* q, uint16_t* out, float* lse, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Spike drain + promotion                                                  */
 /* ------------------------------------------------------------------------ */
 
