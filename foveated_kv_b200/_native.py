@@ -44,12 +44,17 @@ class DecodeShape(C.Structure):
                 ("test_flags", C.c_int32)]
 
 
+def _strides(*names):
+    """Fields of int64 strides (sequence, token, head), flat: ctypes fills them faster than arrays."""
+    return [(f"{n}_{s}", C.c_int64) for n in names for s in ("seq", "tok", "head")]
+
+
 class RotaryShape(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("B", "S", "Hq", "Hk", "D", "rot", "bf16", "interleaved",
                                          "inverse", "pos64")] + \
-               [("amplitude", C.c_float), ("reserved", C.c_int32)] + \
-               [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "q_out_stride",
-                                             "k_out_stride")] + [("pos_stride", C.c_int64 * 2)]
+               [("amplitude", C.c_float), ("reserved", C.c_int32),
+                ("pos_seq", C.c_int64), ("pos_tok", C.c_int64)] + \
+               _strides("q", "q_out", "k", "k_out")
 
 
 class PagedCache(C.Structure):
@@ -60,11 +65,10 @@ class PagedCache(C.Structure):
 
 
 class PagedNew(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "q", "q_out", "cu_new", "inv_freq")] + \
-               [(n, C.c_int64 * 3) for n in ("k_stride", "v_stride", "q_stride",
-                                             "q_out_stride")] + \
-               [(n, C.c_int32) for n in ("T", "n_uniform", "Hq", "rot", "interleaved")] + \
-               [("amplitude", C.c_float)]
+    _fields_ = [(n, C.c_int32) for n in ("T", "n_uniform", "Hq", "rot", "interleaved")] + \
+               [("amplitude", C.c_float)] + \
+               [(n, C.c_void_p) for n in ("cu_new", "inv_freq", "k", "v", "q", "q_out")] + \
+               _strides("k", "v", "q", "q_out")
 
 
 FKV_TEST_STALL = 1
@@ -139,6 +143,8 @@ def load(path: str = None):
     FKV_LIBRARY in the environment names another build of the library (for
     A/B timing of builds; entry points it lacks raise when used)."""
     global _lib
+    if _lib is not None:
+        return _lib
     path = path or os.environ.get("FKV_LIBRARY") or LIB_PATH
     with _lock:
         if _lib is not None:

@@ -31,7 +31,7 @@ import torch
 from . import _native
 from .cache import FoveatedKVCache, compress_layer
 from .config import TierConfig
-from .rotary import check_frequencies, on_device, refuse_grad, rows16
+from .rotary import check_frequencies, on_device, out16, refuse_grad, rows16
 
 _F16 = torch.float16
 _BF16 = torch.bfloat16
@@ -41,39 +41,44 @@ BAD_PAGE, BAD_POSITION = 1, 2
 
 
 def _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dtype):
-    """The checked descriptor of the pages; dtype is that of the tensors beside them."""
-    dev, kind = k_pages.device, k_pages.dtype
-    if not k_pages.is_cuda:
+    """(descriptor of the checked pages, device index); dtype is that of the
+    tensors beside the pages."""
+    index, kind, shape = k_pages.get_device(), k_pages.dtype, k_pages.shape
+    if index < 0:
         raise ValueError(f"{who}: pages must be CUDA tensors")
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype is not kind or v_pages.device != dev \
-            or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not kind or v_pages.get_device() != index \
+            or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError(f"{who}: k_pages and v_pages must be contiguous (P, Hk, page, D) of one type and device")
     if dtype is not _F16 and dtype is not _BF16:
         raise ValueError(f"{who}: {dtype} beside the pages, expected float16 or bfloat16")
-    fp8 = kind is _F8
-    if not fp8 and kind is not dtype:
-        raise ValueError(f"{who}: pages of {kind} beside {dtype}, expected the same type or float8_e4m3fn pages")
-    P, Hk, page, D = k_pages.shape
-    if fp8:
+    P, Hk, page, D = shape
+    if kind is _F8:
         for s in (k_scale, v_scale):
-            if s is None or s.dtype is not torch.float32 or s.device != dev or s.shape != (P, Hk, page) \
+            if s is None or s.dtype is not torch.float32 or s.get_device() != index or s.shape != (P, Hk, page) \
                     or not s.is_contiguous():
                 raise ValueError(f"{who}: float8 pages need contiguous float32 k_scale and v_scale (P, Hk, page)")
-    elif k_scale is not None or v_scale is not None:
-        raise ValueError(f"{who}: scales go with float8 pages only")
-    if table.dtype is not _I32 or table.dim() != 2 or table.device != dev or lens.dtype is not _I32 \
-            or lens.device != dev or lens.shape != table.shape[:1] or not lens.is_contiguous():
-        raise ValueError(f"{who}: table must be int32 (B, W) and lens contiguous int32 (B,) on {dev}")
-    B, W = table.shape
-    stride = table.stride(0) if B > 1 else W
-    if (W > 1 and table.stride(1) != 1) or stride < W:
+        fp8, ks, vs = True, k_scale.data_ptr(), v_scale.data_ptr()
+    else:
+        if kind is not dtype:
+            raise ValueError(f"{who}: pages of {kind} beside {dtype}, expected the same type or float8_e4m3fn pages")
+        if k_scale is not None or v_scale is not None:
+            raise ValueError(f"{who}: scales go with float8 pages only")
+        fp8, ks, vs = False, None, None
+    ts, st = table.shape, table.stride()
+    if len(ts) != 2 or table.dtype is not _I32 or lens.dtype is not _I32 or table.get_device() != index \
+            or lens.get_device() != index or lens.shape != ts[:1] or not lens.is_contiguous():
+        raise ValueError(f"{who}: table must be int32 (B, W) and lens contiguous int32 (B,) on cuda:{index}")
+    B, W = ts
+    stride = st[0] if B > 1 else W
+    if (W > 1 and st[1] != 1) or stride < W:
         raise ValueError(f"{who}: a row of table must be contiguous, and rows must not overlap")
-    if status is not None and (status.dtype is not _I32 or status.device != dev or status.numel() != 1):
-        raise ValueError(f"{who}: status must be one int32 on {dev}")
-    return _native.PagedCache(
-        k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr() if fp8 else None,
-        v_scale.data_ptr() if fp8 else None, table.data_ptr(), lens.data_ptr(),
-        None if status is None else status.data_ptr(), B, Hk, D, page, P, W, stride, fp8, dtype is _BF16)
+    word = None
+    if status is not None:
+        if status.dtype is not _I32 or status.get_device() != index or status.numel() != 1:
+            raise ValueError(f"{who}: status must be one int32 on cuda:{index}")
+        word = status.data_ptr()
+    return _native.PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(), lens.data_ptr(), word,
+                              B, Hk, D, page, P, W, stride, fp8, dtype is _BF16), index
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -99,53 +104,50 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     reads back as NaN.
     """
     who = "paged_append"
-    dt, dev, nd = k.dtype, k_pages.device, k.dim()
+    dt, shape = k.dtype, k.shape
     refuse_grad(who, k, v, q)
-    c = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dt)
-    if v.shape != k.shape or nd not in (3, 4) or (nd == 4 and cu_new is not None) \
-            or k.shape[1] != c.Hk or k.shape[-1] != c.D:
-        raise ValueError(f"{who}: k {tuple(k.shape)} and v {tuple(v.shape)} must be (tokens, {c.Hk}, {c.D}), "
-                         f"or (B, {c.Hk}, n, {c.D}) without cu_new")
-    n = _native.PagedNew()
-    T = k.shape[0]
+    c, index = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dt)
+    nd, Hk, D = len(shape), k_pages.shape[1], k_pages.shape[3]
+    if v.shape != shape or nd not in (3, 4) or (nd == 4 and cu_new is not None) or shape[1] != Hk or shape[-1] != D:
+        raise ValueError(f"{who}: k {tuple(shape)} and v {tuple(v.shape)} must be (tokens, {Hk}, {D}), "
+                         f"or (B, {Hk}, n, {D}) without cu_new")
+    T, B, n, cu = shape[0], table.shape[0], 0, None
     if cu_new is not None:
-        if cu_new.dtype is not _I32 or cu_new.device != dev or cu_new.shape != (c.B + 1,) or not cu_new.is_contiguous():
-            raise ValueError(f"{who}: cu_new must be contiguous int32 (B + 1,) on {dev}")
-        n.cu_new = cu_new.data_ptr()
+        if cu_new.dtype is not _I32 or cu_new.get_device() != index or cu_new.shape != (B + 1,) \
+                or not cu_new.is_contiguous():
+            raise ValueError(f"{who}: cu_new must be contiguous int32 (B + 1,) on cuda:{index}")
+        cu = cu_new.data_ptr()
     else:
-        if T != c.B:
-            raise ValueError(f"{who}: k holds {T} sequences, the table {c.B}")
-        n.n_uniform = k.shape[2] if nd == 4 else 1
-        T *= n.n_uniform
-    n.T = T
-    if (q is None) != (inv_freq is None) and inv_freq is None:
-        raise ValueError(f"{who}: q is only rotated; pass inv_freq with it")
+        if T != B:
+            raise ValueError(f"{who}: k holds {T} sequences, the table {B}")
+        n = shape[2] if nd == 4 else 1
+        T *= n
+    rot, freq = 0, None
     if inv_freq is not None:
-        check_frequencies(who, inv_freq, dev)
-        n.rot, n.inv_freq = 2 * inv_freq.numel(), inv_freq.data_ptr()
-        n.interleaved, n.amplitude = interleaved, amplitude
-    rows = [("k", k, n.k_stride), ("v", v, n.v_stride)]
+        check_frequencies(who, inv_freq, index)
+        rot, freq = 2 * inv_freq.numel(), inv_freq.data_ptr()
+    k, k_st = rows16(who, "k", k, dt, index)
+    v, v_st = rows16(who, "v", v, dt, index)
+    Hq, q_ptr, qo_ptr, q_st, qo_st = 0, None, None, (0, 0, 0), (0, 0, 0)
     if q is not None:
-        if q.dim() != nd or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
-            raise ValueError(f"{who}: q {tuple(q.shape)} does not go with k {tuple(k.shape)}")
-        n.Hq = q.shape[1]
+        if inv_freq is None:
+            raise ValueError(f"{who}: q is only rotated; pass inv_freq with it")
+        if len(q.shape) != nd or q.shape[0] != shape[0] or q.shape[2:] != shape[2:]:
+            raise ValueError(f"{who}: q {tuple(q.shape)} does not go with k {tuple(shape)}")
+        Hq = q.shape[1]
+        q, q_st = rows16(who, "q", q, dt, index)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=dt, device=dev)
-        elif q_out.shape != q.shape or rows16(who, "q_out", q_out, dt, dev) is not q_out \
-                or any(m > 1 and s == 0 for m, s in zip(q_out.shape, q_out.stride())):
-            raise ValueError(f"{who}: q_out has another shape, or is not 8-byte aligned rows with strides of a "
-                             "multiple of 4 elements")
-        rows += [("q", q, n.q_stride), ("q_out", q_out, n.q_out_stride)]
+            q_out, qo_st = rows16(who, "q_out", torch.empty_like(q), dt, index)
+        else:
+            q_out, qo_st = out16(who, "q_out", q_out, q, index)
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError(f"{who}: q_out without q")
-    keep = []
-    for name, t, f in rows:
-        t = rows16(who, name, t, dt, dev)
-        st = t.stride()
-        f[:] = (st[0], st[2], st[1]) if nd == 4 else (st[0], 0 if cu_new is None else st[0], st[1])
-        setattr(n, name, t.data_ptr())
-        keep.append(t)
-    _native.check(on_device(dev, _native.load().fkv_paged_append, C.byref(c), C.byref(n)), "fkv_paged_append")
+    if cu is None and nd == 3:               # one token per sequence: its row is the sequence's
+        k_st, v_st, q_st, qo_st = ((x[1], 0, x[2]) for x in (k_st, v_st, q_st, qo_st))
+    new = _native.PagedNew(T, n, Hq, rot, interleaved, amplitude, cu, freq, k.data_ptr(), v.data_ptr(), q_ptr, qo_ptr,
+                           *k_st, *v_st, *q_st, *qo_st)
+    _native.check(on_device(index, _native.load().fkv_paged_append, C.byref(c), C.byref(new)), "fkv_paged_append")
     return q_out
 
 
@@ -158,13 +160,13 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     who = "paged_read"
     if dtype is None:
         dtype = _F16 if k_pages.dtype is _F8 else k_pages.dtype
-    c = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dtype)
+    c, index = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dtype)
     if max_len < 0:
         raise ValueError(f"{who}: max_len {max_len}")
     k = torch.empty((c.B, c.Hk, max_len, c.D), dtype=dtype, device=k_pages.device)
     v = torch.empty_like(k)
-    _native.check(on_device(k_pages.device, _native.load().fkv_paged_read, C.byref(c), max_len, k.data_ptr(),
-                            v.data_ptr()), "fkv_paged_read")
+    _native.check(on_device(index, _native.load().fkv_paged_read, C.byref(c), max_len, k.data_ptr(), v.data_ptr()),
+                  "fkv_paged_read")
     return k, v
 
 
@@ -183,14 +185,14 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     replayed as sequences grow within the table.
     """
     who = "paged_attend"
-    dt, dev = q.dtype, k_pages.device
+    dt, shape = q.dtype, q.shape
     refuse_grad(who, q)
-    c = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dt)
-    shape = q.shape
-    if q.device != dev or len(shape) not in (3, 4) or shape[0] != c.B or shape[-1] != c.D \
-            or (len(shape) == 4 and shape[2] != 1) or shape[1] < 1 or shape[1] % c.Hk:
-        raise ValueError(f"{who}: q {tuple(shape)} must be (B, Hq, D) or (B, Hq, 1, D) on {dev} with B {c.B}, "
-                         f"D {c.D} and Hq a multiple of {c.Hk}")
+    c, index = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dt)
+    B, Hk, D = table.shape[0], k_pages.shape[1], k_pages.shape[3]
+    if len(shape) not in (3, 4) or shape[0] != B or shape[-1] != D or shape[1] < 1 or shape[1] % Hk \
+            or (len(shape) == 4 and shape[2] != 1) or q.get_device() != index:
+        raise ValueError(f"{who}: q {tuple(shape)} must be (B, Hq, D) or (B, Hq, 1, D) on cuda:{index} with B {B}, "
+                         f"D {D} and Hq a multiple of {Hk}")
     if window < 0:
         raise ValueError(f"{who}: window {window}")
     Hq = shape[1]
@@ -199,17 +201,21 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     if q.data_ptr() & 15:
         q = q.clone()
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
-    elif out.shape != shape or out.dtype is not dt or out.device != dev or not out.is_contiguous() \
+        out = torch.empty_like(q)
+    elif out.shape != shape or out.dtype is not dt or out.get_device() != index or not out.is_contiguous() \
             or out.data_ptr() & 15:
         raise ValueError(f"{who}: out must be a contiguous, 16-byte aligned tensor like q")
-    lse = torch.empty((c.B, Hq), dtype=torch.float32, device=dev) if return_lse else None
-    lib = _native.load()
-    nbytes = lib.fkv_paged_attend_workspace_bytes(C.byref(c), Hq)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _native.check(on_device(dev, lib.fkv_paged_attend, C.byref(c), Hq, c.D ** -0.5 if scale is None else scale,
-                            window, q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-                            None if ws is None else ws.data_ptr(), nbytes), "fkv_paged_attend")
+    lse = lse_ptr = ws_ptr = None
+    if return_lse:
+        lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device)
+        lse_ptr = lse.data_ptr()
+    lib, ref = _native.load(), C.byref(c)
+    nbytes = lib.fkv_paged_attend_workspace_bytes(ref, Hq)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws_ptr = ws.data_ptr()
+    _native.check(on_device(index, lib.fkv_paged_attend, ref, Hq, D ** -0.5 if scale is None else scale, window,
+                            q.data_ptr(), out.data_ptr(), lse_ptr, ws_ptr, nbytes), "fkv_paged_attend")
     return (out, lse) if return_lse else out
 
 

@@ -24,30 +24,47 @@ def refuse_grad(who: str, *tensors) -> None:
                                  "(call it under torch.no_grad())")
 
 
-def rows16(who: str, name: str, t: torch.Tensor, dtype, device) -> torch.Tensor:
-    """t as 16-bit rows the kernels can address: contiguous heads, 8-byte
-    aligned, strides of a multiple of 4 elements; copied where it is not."""
-    if t.dtype is not dtype or t.device != device:
-        raise ValueError(f"{who}: {name} is {t.dtype} on {t.device}, expected {dtype} on {device}")
+def rows16(who: str, name: str, t: torch.Tensor, dtype, index: int):
+    """(t, strides of its sequence, token and head) as 16-bit rows that the
+    kernels can address: contiguous heads, 8-byte aligned, strides of a
+    multiple of 4 elements; t is copied where it is not so.  t is
+    (B, H, S, D) or (tokens, H, D)."""
+    if t.dtype is not dtype or t.get_device() != index:
+        raise ValueError(f"{who}: {name} is {t.dtype} on {t.device}, expected {dtype} on cuda:{index}")
     st = t.stride()
-    if st[-1] != 1 or t.data_ptr() & 7 or any(s & 3 for s in st[:-1]):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    if len(st) == 3:
+        a, h, d = st
+        s, b = a, 0
+    else:
+        b, h, s, d = st
+    if d != 1 or (b | s | h) & 3 or t.data_ptr() & 7:
+        return rows16(who, name, t.clone(memory_format=torch.contiguous_format), dtype, index)
+    return t, (b, s, h)
 
 
-def on_device(device: torch.device, fn, *args) -> int:
+def out16(who: str, name: str, t: torch.Tensor, like: torch.Tensor, index: int):
+    """The same of a tensor that is written: it must be so already."""
+    if t.shape != like.shape:
+        raise ValueError(f"{who}: {name} is {tuple(t.shape)}, expected {tuple(like.shape)}")
+    r, st = rows16(who, name, t, like.dtype, index)
+    if r is not t or any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"{who}: {name} must be 8-byte aligned rows that do not overlap, with strides of a "
+                         "multiple of 4 elements")
+    return r, st
+
+
+def on_device(index: int, fn, *args) -> int:
     """fn(*args, the device's current stream), with that device current."""
-    i = device.index
-    if torch.cuda.current_device() == i:
-        return fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    with torch.cuda.device(i):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if torch._C._cuda_getDevice() == index:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def check_frequencies(who: str, inv_freq: torch.Tensor, device) -> None:
-    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or inv_freq.device != device \
+def check_frequencies(who: str, inv_freq: torch.Tensor, index: int) -> None:
+    if inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or inv_freq.get_device() != index \
             or not inv_freq.is_contiguous():
-        raise ValueError(f"{who}: inv_freq must be a contiguous float64 vector on {device}")
+        raise ValueError(f"{who}: inv_freq must be a contiguous float64 vector on cuda:{index}")
 
 
 def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None,
@@ -105,56 +122,50 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     (a tensor or pair of them, which may be the inputs themselves).
     """
     who = "apply_rotary"
-    if not q.is_cuda:
+    dt, index, shape = q.dtype, q.get_device(), q.shape
+    if index < 0:
         raise ValueError(f"{who}: q must be a CUDA tensor")
-    dev, dt = q.device, q.dtype
     if dt is not _F16 and dt is not _BF16:
         raise ValueError(f"{who}: q is {dt}, expected float16 or bfloat16")
-    nd = q.dim()
-    if nd not in (3, 4):
-        raise ValueError(f"{who}: q must be (B, H, S, D) or (T, H, D), got {tuple(q.shape)}")
     refuse_grad(who, q, k)
-    shape = q.shape
-    if nd == 4:
+    ps = positions.shape
+    if len(shape) == 4:
         B, Hq, S, D = shape
+        fits = ps == (B, S) or ps == (S,)
+    elif len(shape) == 3:
+        S, Hq, D = shape
+        B = 1
+        fits = ps == (S,)
     else:
-        B, (S, Hq, D) = 1, shape
-    Hk = 0
+        raise ValueError(f"{who}: q must be (B, H, S, D) or (T, H, D), got {tuple(shape)}")
+    pd = positions.dtype
+    if not fits or (pd is not torch.int64 and pd is not torch.int32) or positions.get_device() != index:
+        raise ValueError(f"{who}: positions {tuple(ps)} {pd} do not go with q {tuple(shape)}: int32 or int64 "
+                         "(B, S), (S,) or, packed, (T,), on q's device")
+    check_frequencies(who, inv_freq, index)
+    pst = positions.stride()
+    if len(pst) == 1:
+        pst = (0, pst[0])
+    qo = ko = None
+    if out is not None:
+        qo, ko = (out, None) if isinstance(out, torch.Tensor) else out
+        if qo is None or (ko is None) != (k is None):
+            raise ValueError(f"{who}: out must match (q, k)")
+    q, q_st = rows16(who, "q", q, dt, index)
+    qo, qo_st = rows16(who, "out", torch.empty_like(q), dt, index) if qo is None else out16(who, "out", qo, q, index)
+    Hk, k_ptr, ko_ptr, k_st, ko_st = 0, None, None, (0, 0, 0), (0, 0, 0)
     if k is not None:
-        want = (B, k.shape[1], S, D) if nd == 4 else (S, k.shape[1], D)
-        if tuple(k.shape) != want:
-            raise ValueError(f"{who}: k {tuple(k.shape)} does not go with q {tuple(shape)}")
-        Hk = k.shape[1]
-    if positions.device != dev or positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{who}: positions must be int32 or int64 on {dev}")
-    if tuple(positions.shape) not in (((B, S), (S,)) if nd == 4 else ((S,),)):
-        raise ValueError(f"{who}: positions {tuple(positions.shape)} do not go with q {tuple(shape)}")
-    check_frequencies(who, inv_freq, dev)
-
-    outs = (None, None) if out is None else (out, None) if isinstance(out, torch.Tensor) else tuple(out)
-    if out is not None and (len(outs) != 2 or (outs[1] is None) != (k is None)):
-        raise ValueError(f"{who}: out must match (q, k)")
+        kshape = k.shape
+        if len(kshape) != len(shape) or kshape[-1] != D or kshape[0] != shape[0] \
+                or (len(shape) == 4 and kshape[2] != S):
+            raise ValueError(f"{who}: k {tuple(kshape)} does not go with q {tuple(shape)}")
+        Hk = kshape[1]
+        k, k_st = rows16(who, "k", k, dt, index)
+        ko, ko_st = rows16(who, "out", torch.empty_like(k), dt, index) if ko is None else \
+            out16(who, "out", ko, k, index)
+        k_ptr, ko_ptr = k.data_ptr(), ko.data_ptr()
     sh = _native.RotaryShape(B, S, Hq, Hk, D, 2 * inv_freq.numel(), dt is _BF16, interleaved, inverse,
-                             positions.dtype is torch.int64, amplitude)
-    sh.pos_stride[:] = positions.stride() if positions.dim() == 2 else (0, positions.stride(0) if S else 0)
-    ptrs, res = [], []
-    for name, x, o, fin, fout in (("q", q, outs[0], sh.q_stride, sh.q_out_stride),
-                                  ("k", k, outs[1], sh.k_stride, sh.k_out_stride)):
-        if x is None:
-            ptrs += [None, None]
-            continue
-        x = rows16(who, name, x, dt, dev)
-        if o is None:
-            o = torch.empty(x.shape, dtype=dt, device=dev)
-        elif o.shape != x.shape or rows16(who, "out", o, dt, dev) is not o \
-                or any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
-            raise ValueError(f"{who}: out for {name} has another shape, or is not 8-byte aligned "
-                             "rows with strides of a multiple of 4 elements")
-        for t, f in ((x, fin), (o, fout)):
-            st = t.stride()
-            f[:] = (st[0], st[2], st[1]) if nd == 4 else (0, st[0], st[1])
-        ptrs += [x.data_ptr(), o.data_ptr()]
-        res.append(o)
-    _native.check(on_device(dev, _native.load().fkv_rotary, C.byref(sh), ptrs[0], ptrs[2], positions.data_ptr(),
-                            inv_freq.data_ptr(), ptrs[1], ptrs[3]), "fkv_rotary")
-    return res[0] if k is None else tuple(res)
+                             pd is torch.int64, amplitude, 0, *pst, *q_st, *qo_st, *k_st, *ko_st)
+    _native.check(on_device(index, _native.load().fkv_rotary, C.byref(sh), q.data_ptr(), k_ptr,
+                            positions.data_ptr(), inv_freq.data_ptr(), qo.data_ptr(), ko_ptr), "fkv_rotary")
+    return qo if k is None else (qo, ko)

@@ -326,8 +326,8 @@ typedef struct FkvRotaryShape {
     int32_t pos64;             /* positions are int64; otherwise int32 */
     float amplitude;           /* factor of the rotated part */
     int32_t reserved;
-    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];
     int64_t pos_stride[2];
+    int64_t q_stride[3], q_out_stride[3], k_stride[3], k_out_stride[3];
 } FkvRotaryShape;
 
 /* q and k turned by their tokens' positions, in one launch (no counterpart in
@@ -370,16 +370,16 @@ typedef struct FkvPagedCache {
  * [cu_new[b], cu_new[b + 1]) at t * stride[1], and tokens behind cu_new[B]
  * are padding.  They are the last tokens of their sequences. */
 typedef struct FkvPagedNew {
-    const uint16_t *k, *v;       /* (T, Hk, D) */
-    const uint16_t* q;           /* (T, Hq, D), NULL if Hq == 0 */
-    uint16_t* q_out;             /* rotated queries; zeros for tokens that are not stored */
-    const int32_t* cu_new;
-    const double* inv_freq;      /* rot / 2, as fkv_rotary */
-    int64_t k_stride[3], v_stride[3], q_stride[3], q_out_stride[3];
     int32_t T, n_uniform, Hq;
     int32_t rot;                 /* 0: keys are stored as they come */
     int32_t interleaved;
     float amplitude;
+    const int32_t* cu_new;
+    const double* inv_freq;      /* rot / 2, as fkv_rotary */
+    const uint16_t *k, *v;       /* (T, Hk, D) */
+    const uint16_t* q;           /* (T, Hq, D), NULL if Hq == 0 */
+    uint16_t* q_out;             /* rotated queries; zeros for tokens that are not stored */
+    int64_t k_stride[3], v_stride[3], q_stride[3], q_out_stride[3];
 } FkvPagedNew;
 
 /* Writes the new tokens' keys (rotated by their positions) and values into
