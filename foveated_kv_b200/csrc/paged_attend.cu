@@ -111,22 +111,74 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 template <int D, int KIND>
 struct Geo {
     static constexpr int ES = KIND == FP8 ? 1 : 2;            // bytes of a stored element
-    // 16-token groups of one warp's tile
-    static constexpr int TG = D * ES >= 256 ? 1 : 2;
+    static constexpr int RB = D * ES;                         // bytes of a row
+    static constexpr int TG = RB >= 256 ? 1 : 2;              // 16-token groups of one warp's tile
     static constexpr int UNIT = kWarps * 16 * TG;             // tokens of one CTA step
-    static constexpr int KC = D * ES / 64;                    // 16-byte pieces of a key row per lane
+    static constexpr int KC = RB / 64;                        // 16-byte pieces of a key row per lane
     static constexpr int KE = 16 / ES;                        // elements of a piece
     static constexpr int KS = KE / 4;                         // tensor-core steps of a piece
-    static constexpr int VB = D * ES >= 128 ? 16 : 8;         // bytes of a value piece
-    static constexpr int VC = D * ES / (8 * VB);              // value pieces per lane and token
+    static constexpr int VB = RB >= 128 ? 16 : 8;             // bytes of a value piece
+    static constexpr int VC = RB / (8 * VB);                  // value pieces per lane and token
     static constexpr int VW = VB / 4;                         // words of a value piece
     static constexpr int VE = VB / ES;                        // elements of a value piece
     static constexpr int MT = D / 16;                         // 16-row tiles of O^T
+    static constexpr int CP = RB / 32;                        // 512-byte copies of a 16-token group
+    // one warp's buffer: 16 TG rows of K, of V, their scales, and which of its
+    // 8-token groups have a page
+    static constexpr int ROWS = 16 * TG;
+    static constexpr int OFF_V = ROWS * RB;
+    static constexpr int OFF_S = 2 * OFF_V;
+    static constexpr int OFF_L = OFF_S + (KIND == FP8 ? ROWS * 8 : 0);
+    static constexpr int BUF = OFF_L + 16;
+    static constexpr int BUFS = 2;
 };
 
+// Rows sit in shared memory in 128-byte lines whose 16-byte pieces are
+// permuted by the row, so that the lanes of a tensor-core fragment (8 rows of
+// K, or 4 rows and 2 pieces of V, at a time) touch all banks.
+template <int RB>
+__device__ __forceinline__ constexpr int piece_at(int row, int piece) {
+    if (RB >= 128) return row * RB + (piece >> 3) * 128 + (((piece & 7) ^ (row & 7)) << 4);
+    const int line = row >> 1;
+    return line * 128 + ((((row & 1) * 4 + piece) ^ ((line & 3) * 2)) << 4);
+}
+// token (of 8) that row i of a fragment stands for
+template <int RB>
+__device__ __forceinline__ constexpr int token_of(int i) {
+    return RB >= 128 && (i & 1) ? ((i - 1) ^ 4) + 1 : i;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts4(uint32_t a, uint32_t v) {
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+
 // CTAs per SM that a kernel's registers are held to
-template <int D, int NT>
-constexpr int kPerSm = D == 256 || NT == 2 ? 2 : 3;
+template <int D, int NT, int KIND>
+constexpr int kPerSm = Geo<D, KIND>::RB == 512 ? 1 : D == 256 || NT == 2 ? 2 : 3;
 
 // Units of work of sequence b: tokens [lo, len), cut from lo rounded down to 16.
 __device__ __forceinline__ void seq_range(const AttendArgs& a, int b, int& lo, int& len) {
@@ -144,25 +196,42 @@ __device__ __forceinline__ int seq_units(int lo, int len) {
     return len <= lo ? 0 : (len - (lo & ~15) + UNIT - 1) / UNIT;
 }
 
-template <int D, int NT, int KIND>
-struct Smem {
+// the warps' results of one piece of a stream; shares its memory with the buffers
+template <int D, int NT>
+struct Join {
     float o[kWarps][8 * NT][D + 2];
     float m[kWarps][8 * NT], M[kWarps][8 * NT], l[kWarps][8 * NT];
-    int scan[kWarps];
-    int b, prefix, total;
 };
 
 template <int D, int NT, int KIND>
-__global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const __grid_constant__ AttendArgs a) {
+constexpr size_t smem_bytes() {
+    const size_t r = (size_t)kWarps * Geo<D, KIND>::BUFS * Geo<D, KIND>::BUF;
+    return r > sizeof(Join<D, NT>) ? r : sizeof(Join<D, NT>);
+}
+
+template <int D, int NT, int KIND>
+__global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(const __grid_constant__ AttendArgs a) {
     using GG = Geo<D, KIND>;
     constexpr int TG = GG::TG, UNIT = GG::UNIT, KC = GG::KC, KS = GG::KS, VC = GG::VC, VW = GG::VW, MT = GG::MT;
+    constexpr int RB = GG::RB;
     constexpr int HP = 8 * NT;
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    Smem<D, NT, KIND>& sm = *reinterpret_cast<Smem<D, NT, KIND>*>(smem_raw);
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    Join<D, NT>& sm = *reinterpret_cast<Join<D, NT>*>(smem_raw);
+    __shared__ int sh_scan[kWarps], sh_b, sh_prefix;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int B = a.c.B, HS = a.c.Hk * a.HT;
     const bool bf = KIND == BF16 || (KIND == FP8 && a.c.bf16);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // this lane's places in a buffer: fragment rows g of K, rows 2t and 2t + 1 of V
+    const uint32_t bufs = smem_u32(smem_raw) + warp * (GG::BUFS * GG::BUF);
+    const int tok_k = token_of<RB>(g);
+    const uint32_t at_k0 = piece_at<RB>(tok_k, t), at_k1 = RB >= 128 ? piece_at<RB>(tok_k, t + 4) : 0;
+    uint32_t at_v[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int tok = token_of<RB>(2 * t + j);
+        at_v[j] = GG::OFF_V + (GG::VB == 16 ? piece_at<RB>(tok, g) : piece_at<RB>(tok, g >> 1) + (g & 1) * 8);
+    }
 
     // ---- this CTA's run of units ------------------------------------------------------------
     const int per = (B + kThreads - 1) / kThreads;
@@ -178,13 +247,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const _
         const int y = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += y;
     }
-    if (lane == 31) sm.scan[warp] = incl;
+    if (lane == 31) sh_scan[warp] = incl;
     __syncthreads();
     int before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-        before += w < warp ? sm.scan[w] : 0;
-        total += sm.scan[w];
+        before += w < warp ? sh_scan[w] : 0;
+        total += sh_scan[w];
     }
     total *= HS;
     const int excl = before + incl - mine;
@@ -200,8 +269,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const _
             p += n;
             ++b;
         }
-        sm.b = b;
-        sm.prefix = p;
+        sh_b = b;
+        sh_prefix = p;
     }
     // sequences without tokens
     for (int b = blockIdx.x; b < B; b += gridDim.x) {
@@ -218,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const _
     if (a.desc && !a.per_stream && tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     if (u0 >= u1) return;
     __syncthreads();
-    int b = sm.b, prefix = sm.prefix;
+    int b = sh_b, prefix = sh_prefix;
 
     for (int u = u0; u < u1 && b < B;) {
         int lo, len;
@@ -311,92 +380,67 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const _
             l[nt][0] = l[nt][1] = 0.f;
         }
 
-        // page of the 8-token group `lane` of the tile at token t0 (-1: nothing to read)
+        // row of the 8-token group `lane` of the tile at token t0 (~0: nothing to read)
         const int32_t* tab = a.c.table + (int64_t)b * a.c.table_stride;
-        auto page_of = [&](int t0) {
+        auto group_of = [&](int t0) {
             const int tok = t0 + 8 * lane;
-            int pid = -1;
+            uint32_t line = ~0u;
             if (lane < 2 * TG && tok < t_end && tok + 7 >= lo) {
-                pid = tab[tok >> a.pshift];
-                if ((unsigned)pid >= (unsigned)a.c.n_pages) {
+                const int pid = tab[tok >> a.pshift];
+                if ((unsigned)pid >= (unsigned)a.c.n_pages)
                     paged_report(a.c.status, FKV_PAGED_BAD_PAGE);
-                    pid = -1;
-                }
+                else
+                    line = (((uint32_t)pid * a.c.Hk + hk) << a.pshift) + (tok & ((1 << a.pshift) - 1));
             }
-            return pid;
+            return line;
         };
-        const int pmask = (1 << a.pshift) - 1;
-        auto line_of = [&](int pid, int tok) {
-            return (((int64_t)pid * a.c.Hk + hk) << a.pshift) + (tok & pmask);
-        };
-        uint4 kr[TG][2][KC];
-        uint32_t vr[TG][4][VC][VW];
-        float kscale[TG][2], vscale[TG][2];
-        uint32_t live = 0;      // bit 2 tg + half: row g of that 8-token group is a token to attend
-        auto load_k = [&](int t0, int pids) {
-            live = 0;
+        // start the copies of the tile at t0 into `buf`; rows outside [lo, t_end) become zeros
+        auto fetch = [&](uint32_t buf, int t0, uint32_t lines) {
+            if (t0 < t_end) {
 #pragma unroll
-            for (int tg = 0; tg < TG; ++tg)
+                for (int tg = 0; tg < TG; ++tg)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int pid = __shfl_sync(0xffffffffu, pids, 2 * tg + hf);
-                    const int tok = t0 + 16 * tg + 8 * hf + g;
-                    const bool ok = pid >= 0 && tok >= lo && tok < t_end;
-                    live |= (ok ? 1u : 0u) << (2 * tg + hf);
-                    const int64_t line = line_of(pid, tok);
-                    const unsigned char* src = reinterpret_cast<const unsigned char*>(a.c.k_pages) + line * (D * GG::ES) + 16 * t;
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const uint32_t line = __shfl_sync(0xffffffffu, lines, 2 * tg + hf);
+                        const int row0 = 16 * tg + 8 * hf;
+                        const bool have = line != ~0u;
+                        const int64_t at = have ? (int64_t)((uint64_t)line * RB) : 0;
+                        const unsigned char* ks = reinterpret_cast<const unsigned char*>(a.c.k_pages) + at;
+                        const unsigned char* vs = reinterpret_cast<const unsigned char*>(a.c.v_pages) + at;
 #pragma unroll
-                    for (int cc = 0; cc < KC; ++cc) {
-                        kr[tg][hf][cc] = make_uint4(0, 0, 0, 0);
-                        if (ok) kr[tg][hf][cc] = ldg16(src + 64 * cc);
-                    }
-                    if (KIND == FP8) {
-                        kscale[tg][hf] = vscale[tg][hf] = 0.f;
-                        if (ok) {
-                            kscale[tg][hf] = a.c.k_scale[line];
-                            vscale[tg][hf] = a.c.v_scale[line];
+                        for (int i = 0; i < GG::CP / 2; ++i) {
+                            const int row = i * (512 / RB) + lane / (RB / 16), piece = lane % (RB / 16);
+                            const int tok = t0 + row0 + row;
+                            const bool ok = have && tok >= lo && tok < t_end;
+                            const uint32_t dst = buf + row0 * RB + piece_at<RB>(row, piece);
+                            copy16(dst, ks + i * 512 + lane * 16, ok);
+                            copy16(dst + GG::OFF_V, vs + i * 512 + lane * 16, ok);
+                        }
+                        if (KIND == FP8 && lane < 16) {
+                            const int tok = t0 + row0 + (lane & 7);
+                            copy4(buf + GG::OFF_S + (lane >> 3) * (GG::ROWS * 4) + (row0 + (lane & 7)) * 4,
+                                  (lane < 8 ? a.c.k_scale : a.c.v_scale) + (have ? (int64_t)line + (lane & 7) : 0),
+                                  have && tok >= lo && tok < t_end);
                         }
                     }
-                }
-        };
-        auto load_v = [&](int t0, int pids) {
-#pragma unroll
-            for (int tg = 0; tg < TG; ++tg)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int pid = __shfl_sync(0xffffffffu, pids, 2 * tg + (j >> 1));
-                    const int tok = t0 + 16 * tg + 8 * (j >> 1) + 2 * t + (j & 1);
-                    const bool ok = pid >= 0 && tok >= lo && tok < t_end;
-                    const unsigned char* src = reinterpret_cast<const unsigned char*>(a.c.v_pages) +
-                                               line_of(pid, tok) * (D * GG::ES) + GG::VB * g;
-#pragma unroll
-                    for (int c = 0; c < VC; ++c) {
-#pragma unroll
-                        for (int w = 0; w < VW; ++w) vr[tg][j][c][w] = 0;
-                        if (ok) {
-                            if (VW == 4) {
-                                const uint4 x = ldg16(src + 8 * GG::VB * c);
-                                vr[tg][j][c][0] = x.x;
-                                vr[tg][j][c][1] = x.y;
-                                vr[tg][j][c][VW - 2] = x.z;
-                                vr[tg][j][c][VW - 1] = x.w;
-                            } else {
-                                const uint2 x = ldg8(src + 8 * GG::VB * c);
-                                vr[tg][j][c][0] = x.x;
-                                vr[tg][j][c][1] = x.y;
-                            }
-                        }
-                    }
-                }
+                const uint32_t have = __ballot_sync(0xffffffffu, lines != ~0u);
+                if (lane == 0) sts4(buf + GG::OFF_L, have);
+            }
+            copies_commit();
         };
 
         int t0 = t_begin + warp * 16 * TG;
-        int pid_cur = page_of(t0);
-        int pid_nxt = page_of(t0 + UNIT);
-        load_k(t0, pid_cur);
-        load_v(t0, pid_cur);
+        uint32_t buf = 0;      // offset of the tile's buffer
+        uint32_t lines = group_of(t0);
+        fetch(bufs, t0, lines);
+        lines = group_of(t0 + UNIT);
         for (; t0 < t_end; t0 += UNIT) {
-            const int pid_2 = page_of(t0 + 2 * UNIT);
+            copies_wait<0>();
+            __syncwarp();
+            fetch(bufs + (GG::BUF - buf), t0 + UNIT, lines);
+            lines = group_of(t0 + 2 * UNIT);
+            const uint32_t cur = bufs + buf;
+            buf = GG::BUF - buf;
             // scores
             float x[TG][NT][4];
 #pragma unroll
@@ -407,8 +451,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const _
             for (int tg = 0; tg < TG; ++tg)
 #pragma unroll
                 for (int cc = 0; cc < KC; ++cc) {
-                    const uint32_t r0[4] = {kr[tg][0][cc].x, kr[tg][0][cc].y, kr[tg][0][cc].z, kr[tg][0][cc].w};
-                    const uint32_t r1[4] = {kr[tg][1][cc].x, kr[tg][1][cc].y, kr[tg][1][cc].z, kr[tg][1][cc].w};
+                    const uint32_t at = cur + 16 * tg * RB + (cc & 1 ? at_k1 : at_k0) + (cc >> 1) * 128;
+                    const uint4 k0 = lds16(at), k1 = lds16(at + 8 * RB);
+                    const uint32_t r0[4] = {k0.x, k0.y, k0.z, k0.w};
+                    const uint32_t r1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
                     for (int st = 0; st < KS; ++st) {
                         uint32_t a0, a1, a2, a3;
@@ -428,26 +474,31 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const _
                 }
             float av[TG][2];      // log2 of the values' scales
             float top[NT][2], topw[NT][2];
+            const uint32_t have = lds4(cur + GG::OFF_L);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = topw[nt][0] = topw[nt][1] = -INFINITY;
 #pragma unroll
             for (int tg = 0; tg < TG; ++tg)
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const bool ok = (live >> (2 * tg + hf)) & 1;
-                    if (KIND == FP8) av[tg][hf] = lg2(vscale[tg][hf]);
+                    const int row = 16 * tg + 8 * hf + tok_k, tok = t0 + row;
+                    const bool ok = ((have >> (2 * tg + hf)) & 1) && tok >= lo && tok < t_end;
+                    float kscale = 1.f;
+                    if (KIND == FP8) {
+                        kscale = __uint_as_float(lds4(cur + GG::OFF_S + row * 4));
+                        av[tg][hf] = lg2(__uint_as_float(lds4(cur + GG::OFF_S + GG::ROWS * 4 + row * 4)));
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             float& s = x[tg][nt][2 * hf + i];
-                            s *= KIND == FP8 ? qs[nt][i] * kscale[tg][hf] : qs[nt][i];
+                            s *= KIND == FP8 ? qs[nt][i] * kscale : qs[nt][i];
                             s = ok ? s : -INFINITY;
                             top[nt][i] = fmaxf(top[nt][i], s);
                             if (KIND == FP8) topw[nt][i] = fmaxf(topw[nt][i], s + av[tg][hf]);
                         }
                 }
-            load_k(t0 + UNIT, pid_nxt);
             // raise the running maxima when a score passes them by more than kLazy
             bool up = false;
 #pragma unroll
@@ -520,13 +571,25 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const _
 #pragma unroll
             for (int tg = 0; tg < TG; ++tg)
 #pragma unroll
-                for (int c = 0; c < VC; ++c)
+                for (int c = 0; c < VC; ++c) {
+                    // tokens (rows of the fragment) 2t, 2t + 1, 2t + 8, 2t + 9
+                    uint32_t v0[4], v1[4], v2[4], v3[4];
+                    const uint32_t at = cur + 16 * tg * RB + c * 128;
+                    if (VW == 4) {
+                        const uint4 x0 = lds16(at + at_v[0]), x1 = lds16(at + at_v[1]);
+                        const uint4 x2 = lds16(at + at_v[0] + 8 * RB), x3 = lds16(at + at_v[1] + 8 * RB);
+                        v0[0] = x0.x, v0[1] = x0.y, v0[2] = x0.z, v0[3] = x0.w;
+                        v1[0] = x1.x, v1[1] = x1.y, v1[2] = x1.z, v1[3] = x1.w;
+                        v2[0] = x2.x, v2[1] = x2.y, v2[2] = x2.z, v2[3] = x2.w;
+                        v3[0] = x3.x, v3[1] = x3.y, v3[2] = x3.z, v3[3] = x3.w;
+                    } else {
+                        const uint2 x0 = lds8(at + at_v[0]), x1 = lds8(at + at_v[1]);
+                        const uint2 x2 = lds8(at + at_v[0] + 8 * RB), x3 = lds8(at + at_v[1] + 8 * RB);
+                        v0[0] = x0.x, v0[1] = x0.y, v1[0] = x1.x, v1[1] = x1.y;
+                        v2[0] = x2.x, v2[1] = x2.y, v3[0] = x3.x, v3[1] = x3.y;
+                    }
 #pragma unroll
                     for (int w = 0; w < VW; ++w) {
-                        const uint32_t* v0 = vr[tg][0][c];
-                        const uint32_t* v1 = vr[tg][1][c];
-                        const uint32_t* v2 = vr[tg][2][c];
-                        const uint32_t* v3 = vr[tg][3][c];
                         if (KIND == FP8) {
                             uint32_t f[2][4];      // [tokens 2t, 2t+1 | 2t+8, 2t+9][element of the word]
                             e4m3x4_to_h2x2(prmt(v0[w], v1[w], 0x5140), f[0][0], f[0][1]);
@@ -550,11 +613,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT>) attend_kernel(const _
                             }
                         }
                     }
-            load_v(t0 + UNIT, pid_nxt);
-            pid_nxt = pid_2;
+                }
         }
 
         // ---- join the warps -----------------------------------------------------------------------
+        copies_wait<0>();
+        __syncthreads();                 // the buffers' memory changes hands
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -701,7 +765,7 @@ using Kernel = void (*)(const AttendArgs);
 template <int D, int NT, int KIND>
 void entry(Kernel& k, size_t& smem) {
     k = attend_kernel<D, NT, KIND>;
-    smem = sizeof(Smem<D, NT, KIND>);
+    smem = smem_bytes<D, NT, KIND>();
 }
 
 template <int D>
@@ -756,7 +820,7 @@ int make_plan(const FkvPagedCache* c, int Hq, int pshift, int ctas, Plan* p) {
     p->nt = tiles_of(G, c->D);
     p->ht = (G + 8 * p->nt - 1) / (8 * p->nt);
     const int es = c->fp8 ? 1 : 2;
-    p->unit = kWarps * 16 * (c->D * es >= 256 ? 1 : 2);
+    p->unit = kWarps * 16 * (c->D * es >= 256 ? 1 : 2);      // Geo::UNIT
     const int64_t reach = (int64_t)c->width << pshift;
     const int64_t units = (reach + 15 + p->unit - 1) / p->unit;
     const int64_t streams = (int64_t)c->B * c->Hk * p->ht;
