@@ -77,21 +77,23 @@ __device__ __forceinline__ void rotary_apply(float (&x)[8], const Turn& t, bool 
     }
 }
 
-// four 16-bit elements <-> 32 bits
+// 16-bit elements <-> 32 bits
+template <bool BF>
+__device__ __forceinline__ void unpack2(uint32_t u, float* x) {
+    if (BF) {
+        x[0] = __uint_as_float(u << 16);
+        x[1] = __uint_as_float(u & 0xFFFF0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+        x[0] = f.x;
+        x[1] = f.y;
+    }
+}
+
 template <bool BF>
 __device__ __forceinline__ void unpack4(uint2 w, float* x) {
-    const uint32_t u[2] = {w.x, w.y};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if (BF) {
-            x[2 * i] = __uint_as_float(u[i] << 16);
-            x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-        } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        }
-    }
+    unpack2<BF>(w.x, x);
+    unpack2<BF>(w.y, x + 2);
 }
 
 template <bool BF>
