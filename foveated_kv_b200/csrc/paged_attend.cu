@@ -79,6 +79,11 @@ __device__ __forceinline__ float lg2(float x) {
 // 2^(a - b) where b is a maximum over a: 0 for an empty side
 __device__ __forceinline__ float ratio2(float a, float b) { return a == -INFINITY ? 0.f : ex2(a - b); }
 
+// natural log of l 2^m; +inf where a score is (the weights are NaN then)
+__device__ __forceinline__ float log_sum(float m, float l) {
+    return m == INFINITY ? m : (m + log2f(l)) * 0.6931471805599453f;
+}
+
 __device__ __forceinline__ uint4 ldg16(const void* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -89,6 +94,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
+}
+// the next 16-bit numbers below a and b that leave a positive remainder (0 for 0):
+// remainders in (0, 2^-7] of the weight for bf16, [2^-10, 2^-9] for f16
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2_below(float a, float b) {
+    constexpr float f = BF ? 1.f - 0x1p-23f : 1.f - 0x1p-10f;
+    uint32_t r;
+    if (BF) asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b * f), "f"(a * f));
+    else asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b * f), "f"(a * f));
+    return r;
 }
 template <bool BF>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -601,7 +616,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
             // rounding (8 bits of bf16: larger), and the second product is free
             // (1 x 128K f16: 96.4 us with one, 95.9 with two).  8-bit pages take
             // one f16 part, 2^-12 of a weight against the codes' 2^-4: with two,
-            // 64 x 32K goes from 507 to 516 us, 592 to 617 under the power cap
+            // 64 x 32K goes from 507 to 516 us, 592 to 617 under the power cap.
+            // The first part is cut off below the weight, so that both are
+            // positive and an infinite value gives an infinity, not the NaN of
+            // inf - inf (f16: for weights from 2^-14 of the largest; under that
+            // the second part may be zero)
             uint32_t pf[TG][NT][2], pl[TG][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -620,11 +639,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
                             w0 = ex2(x0 + av[tg][hf] - M0);
                             w1 = ex2(x1 + av[tg][hf] - M1);
                         }
-                        const uint32_t hi = pack2<KIND == BF16>(w0, w1);
-                        pf[tg][nt][hf] = transpose8x8(hi);
-                        if (KIND != FP8) {
+                        if (KIND == FP8) {
+                            pf[tg][nt][hf] = transpose8x8(pack2<false>(w0, w1));
+                        } else {
+                            const uint32_t hi = pack2_below<KIND == BF16>(w0, w1);
                             float r[2];
                             unpack2<KIND == BF16>(hi, r);
+                            pf[tg][nt][hf] = transpose8x8(hi);
                             pl[tg][nt][hf] = transpose8x8(pack2<KIND == BF16>(w0 - r[0], w1 - r[1]));
                         }
                     }
@@ -724,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
                 y1 *= f;
                 const int64_t at = (row0 + h) * D + d;
                 *reinterpret_cast<uint32_t*>(a.out + at) = bf ? pack2<true>(y0, y1) : pack2<false>(y0, y1);
-                if (a.lse && d == 0) a.lse[row0 + h] = (mm + log2f(ll)) * 0.6931471805599453f;
+                if (a.lse && d == 0) a.lse[row0 + h] = log_sum(mm, ll);
             } else {
                 const int64_t at = (int64_t)slot * HP + h;
                 *reinterpret_cast<float2*>(a.rec_o + at * D + d) = make_float2(y0, y1);
@@ -845,7 +866,7 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
         const int64_t at = (int64_t)(ds.x + h) * D + d;
         *reinterpret_cast<uint32_t*>(a.out + at) = a.c.bf16 ? pack2<true>(y0 * f, y1 * f) : pack2<false>(y0 * f, y1 * f);
     }
-    if (a.lse && tid == 0) a.lse[ds.x + h] = (m + log2f(ll)) * 0.6931471805599453f;
+    if (a.lse && tid == 0) a.lse[ds.x + h] = log_sum(m, ll);
 }
 
 struct Plan {
