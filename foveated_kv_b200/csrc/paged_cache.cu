@@ -10,6 +10,7 @@
 // so a row with an infinity or a NaN reads back as NaN throughout.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include <cuda_fp8.h>
 
@@ -31,7 +32,8 @@ struct AppendArgs {
     int64_t ks[3], vs[3], qs[3], qos[3];   // strides of (sequence, token, head), elements
     const int32_t* cu_new;
     const double* inv_freq;
-    int n_uniform, Hq, half, pshift;
+    int T, per_block, n_uniform, Hq, half, pshift;
+    FastDiv by_kv, by_q;                   // 2 Hk and Hq
     float amplitude;
 };
 
@@ -41,15 +43,15 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     return lo | (hi << 16);
 }
 
-// One block per new token (and slice of its rows): Hk key rows, Hk value rows
-// and Hq query rows, each taken by D/8 lanes of one warp.
-template <int D, bool BF, bool FP8, bool IL>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
-    constexpr int LPR = D / 8, ROWS = kThreads / LPR;
-    const int u = threadIdx.x % LPR, r = threadIdx.x / LPR;
-    const int t = blockIdx.x;
-    // sequence and position of token t
-    int b, i, n;
+// Where a new token is read and stored.
+struct Place {
+    int64_t k, v, q, q_out;   // element offsets of its rows
+    int64_t line;             // its row of head 0 in the pages; < 0: it is not stored
+    int64_t pos;
+};
+__device__ __forceinline__ Place place_of(const AppendArgs& a, int t) {
+    Place p;
+    int n, b, i;
     bool used = true;
     if (a.cu_new == nullptr) {
         n = a.n_uniform;
@@ -61,93 +63,148 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
             const int mid = (lo + hi + 1) >> 1;
             if (a.cu_new[mid] <= t) lo = mid; else hi = mid - 1;
         }
-        b = lo;
-        used = b < a.c.B && t >= a.cu_new[b];
-        b = min(b, a.c.B - 1);
+        used = lo < a.c.B && t >= a.cu_new[lo];
+        b = min(lo, a.c.B - 1);
         n = a.cu_new[b + 1] - a.cu_new[b];
         i = t - a.cu_new[b];
     }
     const int len = a.c.lens[b];
     used = used && (a.cu_new != nullptr || len != 0);   // an empty slot of a fixed batch
-    const int64_t pos = (int64_t)len - n + i;
-    int pid = -1;
+    p.pos = (int64_t)len - n + i;
+    p.line = -1;
     if (used) {
-        if (pos < 0 || pos >= ((int64_t)a.c.width << a.pshift)) {
+        if (p.pos < 0 || p.pos >= ((int64_t)a.c.width << a.pshift)) {
             paged_report(a.c.status, FKV_PAGED_BAD_POSITION);
         } else {
-            pid = a.c.table[(int64_t)b * a.c.table_stride + (pos >> a.pshift)];
-            if ((unsigned)pid >= (unsigned)a.c.n_pages) {
+            const int pid = a.c.table[(int64_t)b * a.c.table_stride + (p.pos >> a.pshift)];
+            if ((unsigned)pid >= (unsigned)a.c.n_pages)
                 paged_report(a.c.status, FKV_PAGED_BAD_PAGE);
-                pid = -1;
-            }
+            else
+                p.line = (((int64_t)pid * a.c.Hk) << a.pshift) + (p.pos & ((1 << a.pshift) - 1));
         }
     }
-    const bool live = pid >= 0;
-    const RotaryUnit ru = rotary_unit(u, a.half, IL);
-    Turn turn;
-    if (live && ru.turned) {
-        double rate[4];
-        rotary_rates(a.inv_freq, u, rate);
-        turn = rotary_turn(rate, pos, a.amplitude, 1.f);
-    }
-    // strides: a uniform batch is (sequence, token, head); packed rows are (token, head)
+    // a uniform batch has strides of (sequence, token, head), packed rows of (token, head)
     const int64_t sb = a.cu_new ? 0 : b, st = a.cu_new ? t : i;
-    const uint16_t* krow = a.k + sb * a.ks[0] + st * a.ks[1];
-    const uint16_t* vrow = a.v + sb * a.vs[0] + st * a.vs[1];
-    const uint16_t* qrow = a.q + sb * a.qs[0] + st * a.qs[1];
-    uint16_t* qout = a.q_out + sb * a.qos[0] + st * a.qos[1];
-    const int Hk = a.c.Hk, H = 2 * Hk + a.Hq;
-    const int prow = (int)(pos & ((1 << a.pshift) - 1));
-    for (int base = blockIdx.y * ROWS; base < H; base += gridDim.y * ROWS) {
-        const int h = base + r;
-        const bool isq = h >= 2 * Hk, isv = h >= Hk && !isq;
-        const int hh = isq ? h - 2 * Hk : isv ? h - Hk : h;
-        const bool have = live && h < H;
-        uint2 w0 = make_uint2(0, 0), w1 = make_uint2(0, 0);
-        if (have) {
-            const uint16_t* src = isq ? qrow + hh * a.qs[2] : isv ? vrow + hh * a.vs[2] : krow + hh * a.ks[2];
-            w0 = *reinterpret_cast<const uint2*>(src + ru.off0);
-            w1 = *reinterpret_cast<const uint2*>(src + ru.off1);
+    p.k = sb * a.ks[0] + st * a.ks[1];
+    p.v = sb * a.vs[0] + st * a.vs[1];
+    p.q = sb * a.qs[0] + st * a.qs[1];
+    p.q_out = sb * a.qos[0] + st * a.qos[1];
+    return p;
+}
+
+// A block takes up to 8 new tokens (or a slice of one's rows): D/8 lanes of a
+// warp to a row, first the tokens' 2 Hk key and value rows, then their Hq
+// query rows.
+template <int D, bool BF, bool FP8, bool IL, bool W16>
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr int LPR = D / 8, ROWS = kThreads / LPR, N = kRowsAtOnce;
+    extern __shared__ __align__(16) float turns[];       // cosines, sines: [per_block][half] each
+    __shared__ Place places[kMostTokens];
+    const int u = threadIdx.x % LPR, r = threadIdx.x / LPR;
+    const int tok0 = blockIdx.x * a.per_block, count = min(a.per_block, a.T - tok0);
+    if (threadIdx.x < count) places[threadIdx.x] = place_of(a, tok0 + threadIdx.x);
+    __syncthreads();
+    float* cosines = turns;
+    float* sines = turns + a.per_block * a.half;
+    if (a.half) {
+        for (int i = threadIdx.x; i < count * a.half; i += kThreads) {
+            const int k = i / a.half;
+            if (places[k].line >= 0)
+                rotary_pair(a.inv_freq, i - k * a.half, places[k].pos, a.amplitude, cosines[i], sines[i]);
         }
-        float x[8];
-        unpack4<BF>(w0, x);
-        unpack4<BF>(w1, x + 4);
-        if (ru.turned && !isv && have) {
-            rotary_apply(x, turn, IL);
-            w0 = pack4<BF>(x);
-            w1 = pack4<BF>(x + 4);
-        }
-        if (isq) {
-            if (h < H) {                       // zeros behind the last sequence
-                uint16_t* dst = qout + hh * a.qos[2];
-                *reinterpret_cast<uint2*>(dst + ru.off0) = w0;
-                *reinterpret_cast<uint2*>(dst + ru.off1) = w1;
+        __syncthreads();
+    }
+    const RotaryUnit ru = rotary_unit(u, a.half, IL);
+    const int Hk = a.c.Hk, step = gridDim.y * ROWS;
+    const int kv = count * 2 * Hk;
+    for (int base = blockIdx.y * ROWS; base < kv; base += N * step) {
+        uint2 w[N][2];
+        int64_t line[N];
+        int tok[N];
+        bool isk[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = base + j * step + r;
+            const int k = a.by_kv.div(i), h = i - k * 2 * Hk;
+            w[j][0] = w[j][1] = make_uint2(0, 0);
+            line[j] = -1;
+            tok[j] = k;
+            isk[j] = h < Hk;
+            if (i < kv && places[k].line >= 0) {
+                const Place& p = places[k];
+                const int hh = isk[j] ? h : h - Hk;
+                line[j] = p.line + ((int64_t)hh << a.pshift);
+                load_unit<W16>(isk[j] ? a.k + p.k + hh * a.ks[2] : a.v + p.v + hh * a.vs[2], ru, w[j]);
             }
         }
-        const int64_t line = (((int64_t)pid * Hk + hh) << a.pshift) + prow;
-        if (FP8) {
-            // the largest magnitude by its bits: a NaN is above infinity and stays
-            uint32_t top = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-#pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1)
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float most = __uint_as_float(top);
-            most = most < kRowFloor ? kRowFloor : most;
-            if (have && !isq) {
-                const float inv = 448.f / most;
-                uint8_t* dst = reinterpret_cast<uint8_t*>(isv ? a.c.v_pages : a.c.k_pages) + line * D;
-                *reinterpret_cast<uint32_t*>(dst + ru.off0) =
-                    e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-                *reinterpret_cast<uint32_t*>(dst + ru.off1) =
-                    e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-                if (u == 0) (isv ? a.c.v_scale : a.c.k_scale)[line] = most / 448.f;
+        for (int j = 0; j < N; ++j) {
+            const bool turn = isk[j] && ru.turned && line[j] >= 0;
+            float4 c, s;
+            if (turn) {
+                c = *reinterpret_cast<const float4*>(cosines + tok[j] * a.half + 4 * u);
+                s = *reinterpret_cast<const float4*>(sines + tok[j] * a.half + 4 * u);
             }
-        } else if (have && !isq) {
-            uint16_t* dst = reinterpret_cast<uint16_t*>(isv ? a.c.v_pages : a.c.k_pages) + line * D;
-            *reinterpret_cast<uint2*>(dst + ru.off0) = w0;
-            *reinterpret_cast<uint2*>(dst + ru.off1) = w1;
+            if (FP8) {
+                float x[8];
+                unpack4<BF>(w[j][0], x);
+                unpack4<BF>(w[j][1], x + 4);
+                if (turn) rotary_apply(x, c, s, IL);
+                // the largest magnitude by its bits: a NaN is above infinity and stays
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                float most = __uint_as_float(top);
+                most = most < kRowFloor ? kRowFloor : most;
+                if (line[j] >= 0) {
+                    const float inv = 448.f / most;
+                    const uint32_t lo = e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+                    const uint32_t hi = e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+                    uint8_t* dst = reinterpret_cast<uint8_t*>(isk[j] ? a.c.k_pages : a.c.v_pages) + line[j] * D;
+                    if (W16) {
+                        *reinterpret_cast<uint2*>(dst + ru.off0) = make_uint2(lo, hi);
+                    } else {
+                        *reinterpret_cast<uint32_t*>(dst + ru.off0) = lo;
+                        *reinterpret_cast<uint32_t*>(dst + ru.off1) = hi;
+                    }
+                    if (u == 0) (isk[j] ? a.c.k_scale : a.c.v_scale)[line[j]] = most / 448.f;
+                }
+            } else if (line[j] >= 0) {
+                if (turn) turn_unit<BF>(w[j], c, s, IL);
+                store_unit<W16>(reinterpret_cast<uint16_t*>(isk[j] ? a.c.k_pages : a.c.v_pages) + line[j] * D, ru, w[j]);
+            }
+        }
+    }
+    const int nq = count * a.Hq;
+    for (int i0 = blockIdx.y * ROWS + r; i0 < nq; i0 += N * step) {
+        uint2 w[N][2];
+        uint16_t* dst[N];
+        int tok[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = i0 + j * step;
+            const int k = a.by_q.div(i), h = i - k * a.Hq;
+            w[j][0] = w[j][1] = make_uint2(0, 0);           // zeros where a token is not stored
+            dst[j] = nullptr;
+            tok[j] = -1;
+            if (i < nq) {
+                const Place& p = places[k];
+                dst[j] = a.q_out + p.q_out + h * a.qos[2];
+                if (p.line >= 0) {
+                    tok[j] = k;
+                    load_unit<W16>(a.q + p.q + h * a.qs[2], ru, w[j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (dst[j] == nullptr) continue;
+            if (ru.turned && tok[j] >= 0)
+                turn_unit<BF>(w[j], *reinterpret_cast<const float4*>(cosines + tok[j] * a.half + 4 * u),
+                              *reinterpret_cast<const float4*>(sines + tok[j] * a.half + 4 * u), IL);
+            store_unit<W16>(dst[j], ru, w[j]);
         }
     }
 }
@@ -160,70 +217,103 @@ struct ReadArgs {
 
 constexpr int kReadTokens = 64;   // tokens of one (sequence, kv head) per block
 
-// 8 stored elements -> 8 16-bit elements
-template <bool BF, bool FP8>
-__device__ __forceinline__ uint4 read8(const void* pages, const float* scale, int64_t line, int D, int e) {
-    if (!FP8)
-        return *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(pages) + line * D + e);
-    const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(pages) + line * D + e);
-    const float s = scale[line];
-    uint32_t o[4];
+// 8 codes -> 16-bit elements
+template <bool BF>
+__device__ __forceinline__ uint4 widen(const uint2 w, float s) {
     const uint32_t u[2] = {w.x, w.y};
+    uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
             (__nv_fp8x2_storage_t)((u[i >> 1] >> ((i & 1) * 16)) & 0xFFFFu), __NV_E4M3);
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        o[i] = pack2<BF>(f.x * s, f.y * s);
+        r[i] = pack2<BF>(f.x * s, f.y * s);
     }
-    return make_uint4(o[0], o[1], o[2], o[3]);
+    return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// A block reads 64 tokens of one (sequence, kv head), a thread 8 elements of a
+// row at a time, so that a warp's stores fill whole sectors (16 codes and two
+// stores a thread: 24.4 us for 16K tokens), with the loads of several rows of
+// K and V in flight together.
 template <int D, bool BF, bool FP8>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadArgs a) {
-    constexpr int LPR = D / 8, ROWS = kThreads / LPR;
+    constexpr int LPR = D / 8, ROWS = kThreads / LPR, MOST = FP8 ? 8 : 4;
+    constexpr int AT_ONCE = kReadTokens / ROWS < MOST ? kReadTokens / ROWS : MOST;
+    using Piece = std::conditional_t<FP8, uint2, uint4>;
     const int u = threadIdx.x % LPR, r = threadIdx.x / LPR;
     const int64_t bh = blockIdx.x / a.n_chunks;
     const int chunk = (int)(blockIdx.x - bh * a.n_chunks);
     const int b = (int)(bh / a.c.Hk), h = (int)(bh - (int64_t)b * a.c.Hk);
     const int64_t reach = (int64_t)a.c.width << a.pshift;
     const int len = a.c.lens[b];
-    if (len > reach && u == 0 && r == 0 && chunk == 0 && h == 0)
+    if (len > reach && threadIdx.x == 0 && chunk == 0 && h == 0)
         paged_report(a.c.status, FKV_PAGED_BAD_POSITION);
-    const int n = (int)(len < reach ? len : reach);
+    const int n = (int)min((int64_t)min(len, a.max_len), reach);
+    const int32_t* tab = a.c.table + (int64_t)b * a.c.table_stride;
+#pragma unroll 1
+    for (int j0 = 0; j0 < kReadTokens / ROWS; j0 += AT_ONCE) {
+        const int tok0 = chunk * kReadTokens + j0 * ROWS + r;
+        int64_t line[AT_ONCE];
+        Piece kw[AT_ONCE], vw[AT_ONCE];
+        float ks[AT_ONCE], vs[AT_ONCE];
 #pragma unroll
-    for (int j = 0; j < kReadTokens / ROWS; ++j) {
-        const int tok = chunk * kReadTokens + j * ROWS + r;
-        if (tok >= a.max_len) return;
-        uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
-        if (tok < n) {
-            const int pid = a.c.table[(int64_t)b * a.c.table_stride + (tok >> a.pshift)];
-            if ((unsigned)pid < (unsigned)a.c.n_pages) {
-                const int64_t line = (((int64_t)pid * a.c.Hk + h) << a.pshift) + (tok & ((1 << a.pshift) - 1));
-                kw = read8<BF, FP8>(a.c.k_pages, a.c.k_scale, line, D, u * 8);
-                vw = read8<BF, FP8>(a.c.v_pages, a.c.v_scale, line, D, u * 8);
-            } else if (u == 0) {
-                paged_report(a.c.status, FKV_PAGED_BAD_PAGE);
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int tok = tok0 + j * ROWS;
+            line[j] = -1;
+            if (tok < n) {
+                const int pid = tab[tok >> a.pshift];
+                if ((unsigned)pid < (unsigned)a.c.n_pages)
+                    line[j] = (((int64_t)pid * a.c.Hk + h) << a.pshift) + (tok & ((1 << a.pshift) - 1));
+                else if (u == 0)
+                    paged_report(a.c.status, FKV_PAGED_BAD_PAGE);
             }
         }
-        const int64_t o = (bh * a.max_len + tok) * D + u * 8;
-        *reinterpret_cast<uint4*>(a.k + o) = kw;
-        *reinterpret_cast<uint4*>(a.v + o) = vw;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            kw[j] = vw[j] = Piece{};
+            ks[j] = vs[j] = 0.f;
+            if (line[j] >= 0) {
+                const int64_t at = line[j] * LPR + u;
+                kw[j] = reinterpret_cast<const Piece*>(a.c.k_pages)[at];
+                vw[j] = reinterpret_cast<const Piece*>(a.c.v_pages)[at];
+                if (FP8) {
+                    ks[j] = a.c.k_scale[line[j]];
+                    vs[j] = a.c.v_scale[line[j]];
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int tok = tok0 + j * ROWS;
+            if (tok >= a.max_len) continue;
+            const int64_t o = (bh * a.max_len + tok) * LPR + u;
+            if constexpr (FP8) {
+                reinterpret_cast<uint4*>(a.k)[o] = widen<BF>(kw[j], ks[j]);
+                reinterpret_cast<uint4*>(a.v)[o] = widen<BF>(vw[j], vs[j]);
+            } else {
+                reinterpret_cast<uint4*>(a.k)[o] = kw[j];
+                reinterpret_cast<uint4*>(a.v)[o] = vw[j];
+            }
+        }
     }
 }
 
+template <int D, bool BF, bool FP8>
+void launch_append(const AppendArgs& a, dim3 grid, size_t smem, bool il, bool wide, cudaStream_t s) {
+    if (wide) append_kernel<D, BF, FP8, true, true><<<grid, kThreads, smem, s>>>(a);
+    else if (il) append_kernel<D, BF, FP8, true, false><<<grid, kThreads, smem, s>>>(a);
+    else append_kernel<D, BF, FP8, false, false><<<grid, kThreads, smem, s>>>(a);
+}
+
 template <int D>
-void launch_append(const AppendArgs& a, dim3 grid, bool il, cudaStream_t s) {
-    const int mode = (a.c.bf16 ? 4 : 0) | (a.c.fp8 ? 2 : 0) | (il ? 1 : 0);
-    switch (mode) {
-        case 0: append_kernel<D, false, false, false><<<grid, kThreads, 0, s>>>(a); break;
-        case 1: append_kernel<D, false, false, true><<<grid, kThreads, 0, s>>>(a); break;
-        case 2: append_kernel<D, false, true, false><<<grid, kThreads, 0, s>>>(a); break;
-        case 3: append_kernel<D, false, true, true><<<grid, kThreads, 0, s>>>(a); break;
-        case 4: append_kernel<D, true, false, false><<<grid, kThreads, 0, s>>>(a); break;
-        case 5: append_kernel<D, true, false, true><<<grid, kThreads, 0, s>>>(a); break;
-        case 6: append_kernel<D, true, true, false><<<grid, kThreads, 0, s>>>(a); break;
-        default: append_kernel<D, true, true, true><<<grid, kThreads, 0, s>>>(a); break;
+void launch_append(const AppendArgs& a, dim3 grid, size_t smem, bool il, bool wide, cudaStream_t s) {
+    if (a.c.bf16) {
+        if (a.c.fp8) launch_append<D, true, true>(a, grid, smem, il, wide, s);
+        else launch_append<D, true, false>(a, grid, smem, il, wide, s);
+    } else {
+        if (a.c.fp8) launch_append<D, false, true>(a, grid, smem, il, wide, s);
+        else launch_append<D, false, false>(a, grid, smem, il, wide, s);
     }
 }
 
@@ -281,6 +371,8 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
     FKV_REQUIRE(n->cu_new != nullptr || (int64_t)n->n_uniform * c->B == n->T, FKV_ERR_INVALID,
                 "fkv_paged_append: %d tokens are not %d for each of %d sequences", n->T, n->n_uniform, c->B);
     FKV_REQUIRE(n->Hq == 0 || n->rot != 0, FKV_ERR_INVALID, "fkv_paged_append: queries without a rotation");
+    FKV_REQUIRE(c->Hk <= 4096 && n->Hq <= 8192, FKV_ERR_UNSUPPORTED, "fkv_paged_append: %d / %d heads are too many",
+                c->Hk, n->Hq);
     if (n->T == 0 || c->B == 0) return FKV_OK;
     FKV_REQUIRE(n->k && n->v && (n->Hq == 0 || (n->q && n->q_out)) && (n->rot == 0 || n->inv_freq),
                 FKV_ERR_INVALID, "fkv_paged_append: NULL pointer");
@@ -289,6 +381,7 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
     const int64_t* st[4] = {n->k_stride, n->v_stride, n->q_stride, n->q_out_stride};
     int64_t* to[4] = {a.ks, a.vs, a.qs, a.qos};
     const void* ptr[4] = {n->k, n->v, n->q, n->q_out};
+    bool wide = n->rot == 0 || n->interleaved != 0;      // a unit is 16 bytes in a row
     for (int i = 0; i < 4; ++i) {
         if (i >= 2 && n->Hq == 0) {
             to[i][0] = to[i][1] = to[i][2] = 0;
@@ -296,10 +389,12 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
         }
         FKV_REQUIRE((reinterpret_cast<uintptr_t>(ptr[i]) & 7) == 0, FKV_ERR_INVALID,
                     "fkv_paged_append: tensor not 8-byte aligned");
+        wide = wide && (reinterpret_cast<uintptr_t>(ptr[i]) & 15) == 0;
         for (int j = 0; j < 3; ++j) {
             FKV_REQUIRE(st[i][j] % 4 == 0, FKV_ERR_INVALID,
                         "fkv_paged_append: stride %lld is not a multiple of 4 elements", (long long)st[i][j]);
             to[i][j] = st[i][j];
+            wide = wide && st[i][j] % 8 == 0;
         }
     }
     a.k = n->k;
@@ -313,15 +408,20 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
     a.half = n->rot / 2;
     a.pshift = pshift;
     a.amplitude = n->amplitude;
+    a.T = n->T;
     const int rows = kThreads / (c->D / 8);
-    const int passes = (2 * c->Hk + n->Hq + rows - 1) / rows;
-    const int gy = std::min(passes, std::max(1, 592 / n->T));   // few tokens: rows over more blocks
-    const dim3 grid(n->T, gy);
+    const int passes = (std::max(2 * c->Hk, n->Hq) + rows - 1) / rows;
+    // few tokens: their rows are spread over more blocks
+    a.per_block = tokens_per_block(n->T);
+    a.by_kv = FastDiv(2 * (uint32_t)c->Hk);
+    a.by_q = FastDiv((uint32_t)std::max(1, n->Hq));
+    const dim3 grid((n->T + a.per_block - 1) / a.per_block, std::min(passes, std::max(1, 592 / n->T)));
+    const size_t smem = (size_t)a.per_block * a.half * 2 * sizeof(float);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool il = n->interleaved != 0;
-    if (c->D == 64) launch_append<64>(a, grid, il, s);
-    else if (c->D == 128) launch_append<128>(a, grid, il, s);
-    else launch_append<256>(a, grid, il, s);
+    if (c->D == 64) launch_append<64>(a, grid, smem, il, wide, s);
+    else if (c->D == 128) launch_append<128>(a, grid, smem, il, wide, s);
+    else launch_append<256>(a, grid, smem, il, wide, s);
     FKV_LAUNCH_CHECK();
     return FKV_OK;
 }

@@ -21,56 +21,78 @@ struct RotaryArgs {
     const void* pos;
     int64_t ps[2];                          // strides of (batch, token)
     const double* inv_freq;
-    int S, Hq, Hk, D, half;
-    float amplitude, sign;
+    int64_t tokens;
+    int S, Hq, Hk, D, half, per_block, tok_shift;   // tok_shift >= 0: tokens before heads
+    FastDiv by_heads;
+    float amplitude;
+    float sign;                             // of the sines: -1 turns back
 };
 
-// One block per token (and slice of the heads): thread = (unit u, row r); the
-// unit's sines are computed once and used for every head of its rows.
-template <bool BF, bool IL, bool POS64>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-    const int upr = a.D >> 3;
-    const int rows = kThreads / upr;
+template <bool BF, bool IL, bool W16>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a, bool pos64) {
+    extern __shared__ __align__(16) float turns[];       // cosines, sines: [per_block][half] each
+    const int upr = a.D >> 3, rows = kThreads / upr;
     const int r = threadIdx.x / upr, u = threadIdx.x - r * upr;
-    if (r >= rows) return;
-    const int64_t tok = blockIdx.x;
-    const int64_t b = tok / a.S, s = tok - b * a.S;
-    const RotaryUnit ru = rotary_unit(u, a.half, IL);
-    Turn t;
-    if (ru.turned) {
-        const int64_t pi = b * a.ps[0] + s * a.ps[1];
-        const int64_t pos = POS64 ? reinterpret_cast<const int64_t*>(a.pos)[pi]
-                                  : (int64_t) reinterpret_cast<const int32_t*>(a.pos)[pi];
-        double rate[4];
-        rotary_rates(a.inv_freq, u, rate);
-        t = rotary_turn(rate, pos, a.amplitude, a.sign);
+    const int64_t tok0 = (int64_t)blockIdx.x * a.per_block;
+    const int n = (int)min((int64_t)a.per_block, a.tokens - tok0);
+    float* cosines = turns;
+    float* sines = turns + a.per_block * a.half;
+    for (int i = threadIdx.x; i < n * a.half; i += kThreads) {
+        const int k = i / a.half;
+        const int64_t b = (tok0 + k) / a.S, s = tok0 + k - b * a.S, at = b * a.ps[0] + s * a.ps[1];
+        const int64_t pos = pos64 ? reinterpret_cast<const int64_t*>(a.pos)[at]
+                                  : (int64_t) reinterpret_cast<const int32_t*>(a.pos)[at];
+        float c, sn;
+        rotary_pair(a.inv_freq, i - k * a.half, pos, a.amplitude, c, sn);
+        cosines[i] = c;
+        sines[i] = sn * a.sign;
     }
-    const uint16_t* q = a.q + b * a.qs[0] + s * a.qs[1];
-    const uint16_t* k = a.k + b * a.ks[0] + s * a.ks[1];
-    uint16_t* qo = a.q_out + b * a.qos[0] + s * a.qos[1];
-    uint16_t* ko = a.k_out + b * a.kos[0] + s * a.kos[1];
-    const int H = a.Hq + a.Hk;
-    for (int h = blockIdx.y * rows + r; h < H; h += gridDim.y * rows) {
-        const bool isq = h < a.Hq;
-        const uint16_t* src = isq ? q + h * a.qs[2] : k + (h - a.Hq) * a.ks[2];
-        uint16_t* dst = isq ? qo + h * a.qos[2] : ko + (h - a.Hq) * a.kos[2];
-        const uint2 w0 = *reinterpret_cast<const uint2*>(src + ru.off0);
-        const uint2 w1 = *reinterpret_cast<const uint2*>(src + ru.off1);
-        if (!ru.turned) {
-            *reinterpret_cast<uint2*>(dst + ru.off0) = w0;
-            *reinterpret_cast<uint2*>(dst + ru.off1) = w1;
-            continue;
+    __syncthreads();
+    if (r >= rows) return;
+    const RotaryUnit ru = rotary_unit(u, a.half, IL);
+    const int H = a.Hq + a.Hk, total = n * H;
+    const int step = gridDim.y * rows;
+    // rows in the order of memory: heads of a token, or tokens of a head
+    for (int i0 = blockIdx.y * rows + r; i0 < (a.tok_shift >= 0 ? a.per_block * H : total); i0 += kRowsAtOnce * step) {
+        uint2 w[kRowsAtOnce][2];
+        uint16_t* dst[kRowsAtOnce];
+        int tok[kRowsAtOnce];
+#pragma unroll
+        for (int j = 0; j < kRowsAtOnce; ++j) {
+            const int i = i0 + j * step;
+            int k, h;
+            if (a.tok_shift >= 0) {
+                h = i >> a.tok_shift;
+                k = i & (a.per_block - 1);
+            } else {
+                k = a.by_heads.div(i);
+                h = i - k * H;
+            }
+            dst[j] = nullptr;
+            tok[j] = k;
+            if (k < n && h < H) {
+                const int64_t b = a.S == a.tokens ? 0 : (tok0 + k) / a.S, s = tok0 + k - b * a.S;
+                const uint16_t* src;
+                if (h < a.Hq) {
+                    src = a.q + b * a.qs[0] + s * a.qs[1] + h * a.qs[2];
+                    dst[j] = a.q_out + b * a.qos[0] + s * a.qos[1] + h * a.qos[2];
+                } else {
+                    src = a.k + b * a.ks[0] + s * a.ks[1] + (h - a.Hq) * a.ks[2];
+                    dst[j] = a.k_out + b * a.kos[0] + s * a.kos[1] + (h - a.Hq) * a.kos[2];
+                }
+                load_unit<W16>(src, ru, w[j]);
+            }
         }
-        float x[8];
-        unpack4<BF>(w0, x);
-        unpack4<BF>(w1, x + 4);
-        rotary_apply(x, t, IL);
-        *reinterpret_cast<uint2*>(dst + ru.off0) = pack4<BF>(x);
-        *reinterpret_cast<uint2*>(dst + ru.off1) = pack4<BF>(x + 4);
+#pragma unroll
+        for (int j = 0; j < kRowsAtOnce; ++j) {
+            if (dst[j] == nullptr) continue;
+            if (ru.turned)
+                turn_unit<BF>(w[j], *reinterpret_cast<const float4*>(cosines + tok[j] * a.half + 4 * u),
+                              *reinterpret_cast<const float4*>(sines + tok[j] * a.half + 4 * u), IL);
+            store_unit<W16>(dst[j], ru, w[j]);
+        }
     }
 }
-
-bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }
 
 }  // namespace
 
@@ -85,6 +107,8 @@ extern "C" int fkv_rotary(const FkvRotaryShape* sh, const uint16_t* q, const uin
     FKV_REQUIRE(sh->rot >= 8 && sh->rot <= sh->D && sh->rot % 8 == 0, FKV_ERR_UNSUPPORTED,
                 "fkv_rotary: rotated part %d is not a multiple of 8 within the head dim %d",
                 sh->rot, sh->D);
+    FKV_REQUIRE((int64_t)sh->Hq + sh->Hk <= 8192, FKV_ERR_UNSUPPORTED, "fkv_rotary: %d + %d heads are too many",
+                sh->Hq, sh->Hk);
     const int64_t tokens = (int64_t)sh->B * sh->S;
     FKV_REQUIRE(tokens <= INT_MAX, FKV_ERR_UNSUPPORTED, "fkv_rotary: %lld tokens exceed the grid",
                 (long long)tokens);
@@ -96,17 +120,21 @@ extern "C" int fkv_rotary(const FkvRotaryShape* sh, const uint16_t* q, const uin
     const int64_t* st[4] = {sh->q_stride, sh->k_stride, sh->q_out_stride, sh->k_out_stride};
     int64_t* to[4] = {a.qs, a.ks, a.qos, a.kos};
     const void* ptr[4] = {q, k, q_out, k_out};
+    bool wide = sh->interleaved != 0;
     for (int i = 0; i < 4; ++i) {
         if (((i & 1) ? sh->Hk : sh->Hq) == 0) {
             to[i][0] = to[i][1] = to[i][2] = 0;
             continue;
         }
-        FKV_REQUIRE(aligned8(ptr[i]), FKV_ERR_INVALID, "fkv_rotary: tensor not 8-byte aligned");
+        FKV_REQUIRE((reinterpret_cast<uintptr_t>(ptr[i]) & 7) == 0, FKV_ERR_INVALID,
+                    "fkv_rotary: tensor not 8-byte aligned");
+        wide = wide && (reinterpret_cast<uintptr_t>(ptr[i]) & 15) == 0;
         for (int j = 0; j < 3; ++j) {
             FKV_REQUIRE(st[i][j] % 4 == 0, FKV_ERR_INVALID,
                         "fkv_rotary: stride %lld is not a multiple of 4 elements",
                         (long long)st[i][j]);
             to[i][j] = st[i][j];
+            wide = wide && st[i][j] % 8 == 0;
         }
     }
     a.q = q;
@@ -117,6 +145,7 @@ extern "C" int fkv_rotary(const FkvRotaryShape* sh, const uint16_t* q, const uin
     a.ps[0] = sh->pos_stride[0];
     a.ps[1] = sh->pos_stride[1];
     a.inv_freq = inv_freq;
+    a.tokens = tokens;
     a.S = sh->S;
     a.Hq = sh->Hq;
     a.Hk = sh->Hk;
@@ -126,20 +155,26 @@ extern "C" int fkv_rotary(const FkvRotaryShape* sh, const uint16_t* q, const uin
     a.sign = sh->inverse ? -1.f : 1.f;
     const int rows = kThreads / (sh->D / 8);
     const int passes = (sh->Hq + sh->Hk + rows - 1) / rows;
+    a.per_block = tokens_per_block(tokens);
+    // rows of a block in the order of memory: (B, H, S, D) has a head's tokens together
+    const int64_t* lead = sh->Hq ? a.qs : a.ks;
+    a.tok_shift = -1;
+    if (a.per_block > 1 && lead[1] < lead[2])
+        for (a.tok_shift = 0; (1 << a.tok_shift) < a.per_block;) ++a.tok_shift;
+    a.by_heads = FastDiv((uint32_t)(sh->Hq + sh->Hk));
     // few tokens: their heads are spread over more blocks
     const int gy = (int)std::min<int64_t>(passes, std::max<int64_t>(1, 592 / tokens));
-    const dim3 grid((unsigned)tokens, (unsigned)gy);
+    const dim3 grid((unsigned)((tokens + a.per_block - 1) / a.per_block), (unsigned)gy);
+    const size_t smem = (size_t)a.per_block * a.half * 2 * sizeof(float);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int mode = (sh->bf16 ? 4 : 0) | (sh->interleaved ? 2 : 0) | (sh->pos64 ? 1 : 0);
-    switch (mode) {
-        case 0: rotary_kernel<false, false, false><<<grid, kThreads, 0, s>>>(a); break;
-        case 1: rotary_kernel<false, false, true><<<grid, kThreads, 0, s>>>(a); break;
-        case 2: rotary_kernel<false, true, false><<<grid, kThreads, 0, s>>>(a); break;
-        case 3: rotary_kernel<false, true, true><<<grid, kThreads, 0, s>>>(a); break;
-        case 4: rotary_kernel<true, false, false><<<grid, kThreads, 0, s>>>(a); break;
-        case 5: rotary_kernel<true, false, true><<<grid, kThreads, 0, s>>>(a); break;
-        case 6: rotary_kernel<true, true, false><<<grid, kThreads, 0, s>>>(a); break;
-        default: rotary_kernel<true, true, true><<<grid, kThreads, 0, s>>>(a); break;
+    const bool p64 = sh->pos64 != 0;
+    switch ((sh->bf16 ? 4 : 0) | (sh->interleaved ? 2 : 0) | (wide ? 1 : 0)) {
+        case 0: rotary_kernel<false, false, false><<<grid, kThreads, smem, s>>>(a, p64); break;
+        case 2: rotary_kernel<false, true, false><<<grid, kThreads, smem, s>>>(a, p64); break;
+        case 3: rotary_kernel<false, true, true><<<grid, kThreads, smem, s>>>(a, p64); break;
+        case 4: rotary_kernel<true, false, false><<<grid, kThreads, smem, s>>>(a, p64); break;
+        case 6: rotary_kernel<true, true, false><<<grid, kThreads, smem, s>>>(a, p64); break;
+        default: rotary_kernel<true, true, true><<<grid, kThreads, smem, s>>>(a, p64); break;
     }
     FKV_LAUNCH_CHECK();
     return FKV_OK;

@@ -12,9 +12,11 @@
 // 1e-7 of a turn; in 32 bits it would be whole turns), and only the remainder
 // goes to sincospif in 32 bits.
 //
-// A unit is 4 pairs = 8 elements, the work of one thread on one row: two
-// 8-byte accesses at off0 and off1.  rot is a multiple of 8, so a unit is
-// either turned as a whole or passed through as a whole.
+// A block takes a few tokens: it first puts the sines and cosines of their
+// pairs into shared memory, one pair per thread, then goes over all rows
+// (heads) of the tokens.  A unit is 4 pairs = 8 elements, the work of one
+// thread on one row: at off0 and off1, 4 elements each.  rot is a multiple of
+// 8, so a unit is either turned as a whole or passed through as a whole.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -24,10 +26,6 @@
 #include <cstdint>
 
 namespace fkvdev {
-
-struct Turn {
-    float c[4], s[4];
-};
 
 struct RotaryUnit {
     int off0, off1;   // element offsets of the unit's two groups of 4
@@ -43,37 +41,69 @@ __device__ __forceinline__ RotaryUnit rotary_unit(int u, int half, bool interlea
     return r;
 }
 
-// turns per position of the unit's 4 pairs
-__device__ __forceinline__ void rotary_rates(const double* __restrict__ inv_freq, int u,
-                                             double (&rate)[4]) {
+// x / n by a multiplication: exact while x * n < 2^32 (rows of a block: x is
+// under 8 tokens' rows)
+struct FastDiv {
+    uint32_t n, m;
+    FastDiv() = default;
+    __host__ explicit FastDiv(uint32_t n_) : n(n_), m((uint32_t)((0x100000000ull + n_ - 1) / n_)) {}
+    __device__ __forceinline__ int div(int x) const { return n == 1 ? x : (int)__umulhi((uint32_t)x, m); }
+};
+
+// tokens of a block: as many as leave kMinBlocks blocks, a power of two
+constexpr int kMinBlocks = 148 * 16, kMostTokens = 8;
+inline int tokens_per_block(int64_t tokens) {
+    int p = 1;
+    while (p < kMostTokens && tokens / (2 * p) >= kMinBlocks) p *= 2;
+    return p;
+}
+
+// rows that a thread has in flight: loads come first, since the compiler may
+// not move them over the stores of rows that could be the same memory
+constexpr int kRowsAtOnce = 2;
+
+// cosine and sine (times amplitude) of pair p at position pos
+__device__ __forceinline__ void rotary_pair(const double* __restrict__ inv_freq, int p, int64_t pos,
+                                            float amplitude, float& c, float& s) {
     constexpr double kInv2Pi = 0.15915494309189533577;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rate[i] = inv_freq[4 * u + i] * kInv2Pi;
+    const double turns = (double)pos * (inv_freq[p] * kInv2Pi);
+    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+    c *= amplitude;
+    s *= amplitude;
 }
 
-__device__ __forceinline__ Turn rotary_turn(const double (&rate)[4], int64_t pos, float amplitude,
-                                            float sign) {
-    Turn t;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const double turns = (double)pos * rate[i];
-        const float frac = (float)(turns - rint(turns));
-        float s, c;
-        sincospif(2.f * frac, &s, &c);
-        t.c[i] = c * amplitude;
-        t.s[i] = s * amplitude * sign;
-    }
-    return t;
-}
-
-// x[0..3] are the elements at off0, x[4..7] those at off1
-__device__ __forceinline__ void rotary_apply(float (&x)[8], const Turn& t, bool interleaved) {
+// x[0..3] are the elements at off0, x[4..7] those at off1; c, s of 4 pairs
+__device__ __forceinline__ void rotary_apply(float (&x)[8], const float4 c4, const float4 s4, bool interleaved) {
+    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int ia = interleaved ? 2 * i : i, ib = interleaved ? 2 * i + 1 : 4 + i;
         const float a = x[ia], b = x[ib];
-        x[ia] = fmaf(a, t.c[i], -b * t.s[i]);
-        x[ib] = fmaf(a, t.s[i], b * t.c[i]);
+        x[ia] = fmaf(a, c[i], -b * s[i]);
+        x[ib] = fmaf(a, s[i], b * c[i]);
+    }
+}
+
+// A unit of a row of 16-bit elements.  W16: one 16-byte access (its two groups
+// are neighbours and rows are 16-byte aligned), otherwise two of 8.
+template <bool W16>
+__device__ __forceinline__ void load_unit(const uint16_t* row, const RotaryUnit& u, uint2 (&w)[2]) {
+    if (W16) {
+        const uint4 x = *reinterpret_cast<const uint4*>(row + u.off0);
+        w[0] = make_uint2(x.x, x.y);
+        w[1] = make_uint2(x.z, x.w);
+    } else {
+        w[0] = *reinterpret_cast<const uint2*>(row + u.off0);
+        w[1] = *reinterpret_cast<const uint2*>(row + u.off1);
+    }
+}
+template <bool W16>
+__device__ __forceinline__ void store_unit(uint16_t* row, const RotaryUnit& u, const uint2 (&w)[2]) {
+    if (W16) {
+        *reinterpret_cast<uint4*>(row + u.off0) = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
+    } else {
+        *reinterpret_cast<uint2*>(row + u.off0) = w[0];
+        *reinterpret_cast<uint2*>(row + u.off1) = w[1];
     }
 }
 
@@ -109,6 +139,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <bool BF>
 __device__ __forceinline__ uint2 pack4(const float* x) {
     return make_uint2(pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]));
+}
+
+// the unit turned, in its 16-bit form
+template <bool BF>
+__device__ __forceinline__ void turn_unit(uint2 (&w)[2], const float4 c, const float4 s, bool interleaved) {
+    float x[8];
+    unpack4<BF>(w[0], x);
+    unpack4<BF>(w[1], x + 4);
+    rotary_apply(x, c, s, interleaved);
+    w[0] = pack4<BF>(x);
+    w[1] = pack4<BF>(x + 4);
 }
 
 }  // namespace fkvdev
