@@ -171,6 +171,34 @@ def load(path: str = None):
         return lib
 
 
+_ops = None
+OPS_PATH = os.path.join(_HERE, "_lib", "fkv_ops.so")
+
+
+def ops():
+    """fkv_ops.so (csrc/ops.cpp): the rotary and paged-cache calls, bound to the loaded libfkv."""
+    global _ops
+    if _ops is None:
+        import importlib.machinery
+        import importlib.util
+
+        lib = load()
+        if not os.path.exists(OPS_PATH):
+            raise FkvNativeError(f"fkv_ops.so not found at {OPS_PATH}; build it with "
+                                 "`python -m foveated_kv_b200.build`")
+        try:
+            loader = importlib.machinery.ExtensionFileLoader("fkv_ops", OPS_PATH)
+            mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("fkv_ops", loader))
+            loader.exec_module(mod)
+            mod.bind(FkvNativeError, *(C.cast(getattr(lib, n), P).value for n in (
+                "fkv_last_error", "fkv_rotary", "fkv_paged_append", "fkv_paged_read", "fkv_paged_attend",
+                "fkv_paged_attend_workspace_bytes")))
+        except (ImportError, AttributeError) as e:
+            raise FkvNativeError(f"failed to load {OPS_PATH}: {e}") from e
+        _ops = mod
+    return _ops
+
+
 def check(rc: int, what: str):
     if rc < 0:
         msg = load().fkv_last_error().decode(errors="replace")

@@ -17,15 +17,23 @@
 // are read in every call, so the workspace needs no initialisation, and two
 // calls share nothing.
 //
-// Tile.  One warp takes 16 tokens at a time straight from global memory to
-// registers, each lane in 16-byte pieces in the order in which the tensor
-// core wants them (row = lane / 4 = g, quad = lane % 4 = t):
+// Tile.  One warp takes 16 or 32 tokens at a time, each lane in 16-byte pieces in
+// the order in which the tensor core wants them (row = lane / 4 = g, quad =
+// lane % 4 = t):
 //   S^T (16 tok x 8 heads)  = K (16 x D) . Q^T      lane: rows g, g + 8 of K
 //   O^T (D x 8 heads)      += V^T (D x 16) . P^T    lane: rows 2t, 2t+1, 2t+8, 2t+9 of V
 // The products' inner order is free, so the 16-byte pieces of K pair with the
 // same pieces of Q; V rows pair up by byte permutes; P^T comes from S^T by an
-// 8x8 transpose across lanes.  K and V of the next tile are in flight while
-// this one is computed.
+// 8x8 transpose across lanes.  mma.sync, not tcgen05: with up to 8 heads a
+// tile the products are 13 % of the tensor pipe's time, and every byte is used
+// once, so the bound is memory.
+//
+// Loads.  16-bit pages go straight from global memory to registers, K of the
+// next tile in flight during the softmax and V, V during the next K (1 x 64K of
+// 8 kv heads, f16: 50.9 us, through shared memory 53.1; 33 ragged windows 46 /
+// 55).  8-bit pages need twice the instructions a byte, and registers could not
+// hide them: they go by 16-byte asynchronous copies through two buffers a warp
+// in shared memory (64 x 32K: 667 us direct, 505 through buffers).
 //
 // 8-bit rows: codes become f16 exactly.  A key's scale multiplies its score.
 // A value's scale joins the exponent: w_n = exp2(x_n + log2 s_n - M) with a
@@ -120,21 +128,27 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Which units a CTA takes.  SMs differ: with equal shares some finished 15 %
-// after the mean (1M fp8 tokens: mean 305 us, last 370).  So a call with much
-// work deals its units in falling shares: 90 % to the first wave of CTAs, the
-// rest to CTAs that start as others end; with more work 80 %, 13 % and the
-// rest.  A CTA costs a start and a record, so small calls stay with one wave
-// (measured with 1 / 2 / 3 waves, us: 1 x 16K of 32 kv heads f16, 18 units a
-// CTA: 51.7 / 52.2 / 56.0; 16 x 8K f16, 27 units: 77.3 / 74.9 / 76.3; 1 x 512K
-// fp8, 74 units: 193 / 180 / 183; 64 x 32K fp8, 221 units: 552 / 507 / 501).
-// The shares go by the CTA's number alone, so pieces and results do not depend
-// on who was faster.
+// Which units a CTA takes: equal shares, or, for 8-bit pages and much work,
+// falling ones, 90 % to the first wave of CTAs and the rest to CTAs that start
+// as others end; with more work 80 %, 13 % and the rest.  With equal shares of
+// 8-bit pages some SMs finished 15 % after the mean (1M tokens: mean 305 us,
+// last 370), while a CTA costs a start and a record (1 / 2 / 3 waves, us: 1 x
+// 128K fp8, 18 units a CTA: 56.0 / 60.6 / 64.9; 1 x 256K, 37 units: 104 / 99 /
+// 104; 1 x 512K, 74: 193 / 180 / 183; 64 x 32K, 221: 552 / 507 / 501).  16-bit
+// pages gain nothing (64 x 4K f16, 54 units: 129 / 132 / 135; 64 x 16K, 222:
+// 474 / 476 / 475).  The shares go by the CTA's number alone, so pieces and
+// results do not depend on who was faster.
 constexpr int kMostWaves = 3;
 constexpr int kUnits2 = 24, kUnits3 = 100;   // units a CTA from which 2 and 3 waves pay
 struct Deal {
     int wave, total, r[kMostWaves];
+    Deal() = default;
     __device__ Deal(int total_, int wave_, int waves) : wave(wave_), total(total_) {
+        if (waves == 1) {
+            r[0] = (total + wave - 1) / wave;
+            r[1] = r[2] = 0;
+            return;
+        }
         const int each = total / wave;
         waves = min(waves, each < kUnits2 ? 1 : each < kUnits3 ? 2 : 3);
         int left = total;
@@ -183,6 +197,7 @@ struct Geo {
     static constexpr int VE = VB / ES;                        // elements of a value piece
     static constexpr int MT = D / 16;                         // 16-row tiles of O^T
     static constexpr int CP = RB / 32;                        // 512-byte copies of a 16-token group
+    static constexpr bool DIRECT = KIND != FP8;               // straight to registers
     // one warp's buffer: 16 TG rows of K, of V, their scales, and which of its
     // 8-token groups have a page
     static constexpr int ROWS = 16 * TG;
@@ -242,7 +257,7 @@ __device__ __forceinline__ void sts4(uint32_t a, uint32_t v) {
 
 // CTAs per SM that a kernel's registers are held to
 template <int D, int NT, int KIND>
-constexpr int kPerSm = Geo<D, KIND>::RB == 512 ? 1 : D == 256 || NT == 2 ? 2 : 3;
+constexpr int kPerSm = D == 256 || NT == 2 ? 2 : 3;
 
 // Units of work of sequence b: tokens [lo, len), cut from lo rounded down to 16.
 __device__ __forceinline__ void seq_range(const AttendArgs& a, int b, int& lo, int& len) {
@@ -269,7 +284,7 @@ struct Join {
 
 template <int D, int NT, int KIND>
 constexpr size_t smem_bytes() {
-    const size_t r = (size_t)kWarps * Geo<D, KIND>::BUFS * Geo<D, KIND>::BUF;
+    const size_t r = Geo<D, KIND>::DIRECT ? 0 : (size_t)kWarps * Geo<D, KIND>::BUFS * Geo<D, KIND>::BUF;
     return r > sizeof(Join<D, NT>) ? r : sizeof(Join<D, NT>);
 }
 
@@ -278,6 +293,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
     using GG = Geo<D, KIND>;
     constexpr int TG = GG::TG, UNIT = GG::UNIT, KC = GG::KC, KS = GG::KS, VC = GG::VC, VW = GG::VW, MT = GG::MT;
     constexpr int RB = GG::RB;
+    constexpr bool DIRECT = GG::DIRECT;
     constexpr int HP = 8 * NT;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Join<D, NT>& sm = *reinterpret_cast<Join<D, NT>*>(smem_raw);
@@ -290,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // this lane's places in a buffer: fragment rows g of K, rows 2t and 2t + 1 of V
     const uint32_t bufs = smem_u32(smem_raw) + warp * (GG::BUFS * GG::BUF);
-    const int tok_k = token_of<RB>(g);
+    const int tok_k = DIRECT ? g : token_of<RB>(g);
     const uint32_t at_k0 = piece_at<RB>(tok_k, t), at_k1 = RB >= 128 ? piece_at<RB>(tok_k, t + 4) : 0;
     uint32_t at_c[GG::CP / 2], at_v[2];      // 512-byte copies of 8 rows
 #pragma unroll
@@ -302,43 +318,64 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
     }
 
     // ---- this CTA's run of units ------------------------------------------------------------
-    const int per = (B + kThreads - 1) / kThreads;
-    int mine = 0;
-    for (int b = tid * per; b < min(B, (tid + 1) * per); ++b) {
+    Deal deal;
+    int u0, u1;
+    if (a.desc == nullptr) {               // a CTA per stream
         int lo, len;
+        const int b = blockIdx.x / HS;
         seq_range(a, b, lo, len);
-        mine += seq_units<UNIT>(lo, len);
-    }
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) sh_scan[warp] = incl;
-    __syncthreads();
-    int before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        before += w < warp ? sh_scan[w] : 0;
-        total += sh_scan[w];
-    }
-    total *= HS;
-    const int excl = before + incl - mine;
-    const Deal deal(total, a.wave, a.waves);
-    const int u0 = deal.begin(blockIdx.x), u1 = deal.begin(blockIdx.x + 1);
-    if (u0 < u1 && u0 >= excl * HS && u0 < (excl + mine) * HS) {
-        int b = tid * per, p = excl;
-        while (b + 1 < B) {
+        const int n = seq_units<UNIT>(lo, len);
+        u0 = (blockIdx.x - b * HS) * n;
+        u1 = u0 + n;
+        if (tid == 0) {
+            sh_b = b;
+            sh_prefix = 0;
+        }
+    } else {
+        const int per = (B + kThreads - 1) / kThreads;
+        int mine = 0;
+        for (int b = tid * per; b < min(B, (tid + 1) * per); ++b) {
             int lo, len;
             seq_range(a, b, lo, len);
-            const int n = seq_units<UNIT>(lo, len);
-            if (u0 < (p + n) * HS) break;
-            p += n;
-            ++b;
+            mine += seq_units<UNIT>(lo, len);
         }
-        sh_b = b;
-        sh_prefix = p;
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) sh_scan[warp] = incl;
+        __syncthreads();
+        int before = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            before += w < warp ? sh_scan[w] : 0;
+            total += sh_scan[w];
+        }
+        total *= HS;
+        const int excl = before + incl - mine;
+        deal = Deal(total, a.wave, a.waves);
+        if (a.waves == 1) {
+            u0 = min((int64_t)deal.r[0] * blockIdx.x, (int64_t)total);
+            u1 = min(u0 + deal.r[0], total);
+        } else {
+            u0 = deal.begin(blockIdx.x);
+            u1 = deal.begin(blockIdx.x + 1);
+        }
+        if (u0 < u1 && u0 >= excl * HS && u0 < (excl + mine) * HS) {
+            int b = tid * per, p = excl;
+            while (b + 1 < B) {
+                int lo, len;
+                seq_range(a, b, lo, len);
+                const int n = seq_units<UNIT>(lo, len);
+                if (u0 < (p + n) * HS) break;
+                p += n;
+                ++b;
+            }
+            sh_b = b;
+            sh_prefix = p;
+        }
     }
     // sequences without tokens
     for (int b = blockIdx.x; b < B; b += gridDim.x) {
@@ -349,10 +386,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
             reinterpret_cast<uint32_t*>(a.out)[(int64_t)b * a.Hq * D / 2 + i] = 0;
         if (a.lse)
             for (int i = tid; i < a.Hq; i += kThreads) a.lse[(int64_t)b * a.Hq + i] = -INFINITY;
-        if (a.desc && a.per_stream)
+        if (a.per_stream)
             for (int i = tid; i < HS; i += kThreads) a.desc[b * HS + i] = make_int4(0, 0, 0, 0);
     }
-    if (a.desc && !a.per_stream && tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (a.desc != nullptr && !a.per_stream && tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     if (u0 >= u1) return;
     __syncthreads();
     int b = sh_b, prefix = sh_prefix;
@@ -367,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
             continue;
         }
         const int rel = u - prefix * HS, stream = rel / nu, chunk = rel - stream * nu;
-        const int hk = stream / a.HT, ht = stream - hk * a.HT;
+        const int hk = a.HT == 1 ? stream : stream / a.HT, ht = stream - hk * a.HT;
         const int s_begin = u - chunk, s_end = s_begin + nu;       // the stream's units
         const int chunk_end = min(nu, chunk + (u1 - u));
         const int base = lo & ~15;
@@ -447,10 +484,69 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
             copies_commit();
         };
 
+        // DIRECT: the lane's pieces of the tile at t0, rows g of K and 2t, 2t + 1 of
+        // V of every 8-token group; rows outside [lo, t_end) become zeros
+        uint4 kr[TG][2][KC], vr[TG][4][VC];
+        uint32_t live = 0;     // rows g to attend, a bit for each 8-token group
+        auto is_full = [&](int t0, uint32_t lines) {
+            return __all_sync(0xffffffffu, lines != ~0u || lane >= 2 * TG) && t0 >= lo && t0 + GG::ROWS <= t_end;
+        };
+        auto load_k = [&](int t0, uint32_t lines) {
+            const bool full = is_full(t0, lines);
+            live = ~0u;
+#pragma unroll
+            for (int k = 0; k < 2 * TG; ++k) {
+                const uint32_t line = __shfl_sync(0xffffffffu, lines, k);
+                const unsigned char* src = reinterpret_cast<const unsigned char*>(a.c.k_pages) +
+                                           ((uint64_t)line * RB + g * RB + 16 * t);
+                if (full) {
+#pragma unroll
+                    for (int cc = 0; cc < KC; ++cc) kr[k >> 1][k & 1][cc] = ldg16(src + 64 * cc);
+                } else {
+                    const int tok = t0 + 8 * k + g;
+                    const bool ok = line != ~0u && tok >= lo && tok < t_end;
+                    if (!ok) live &= ~(1u << k);
+#pragma unroll
+                    for (int cc = 0; cc < KC; ++cc) {
+                        kr[k >> 1][k & 1][cc] = make_uint4(0, 0, 0, 0);
+                        if (ok) kr[k >> 1][k & 1][cc] = ldg16(src + 64 * cc);
+                    }
+                }
+            }
+        };
+        auto load_v = [&](int t0, uint32_t lines) {
+            const bool full = is_full(t0, lines);
+#pragma unroll
+            for (int k = 0; k < 2 * TG; ++k) {
+                const uint32_t line = __shfl_sync(0xffffffffu, lines, k);
+                const unsigned char* src = reinterpret_cast<const unsigned char*>(a.c.v_pages) +
+                                           ((uint64_t)line * RB + 2 * t * RB + GG::VB * g);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int tok = t0 + 8 * k + 2 * t + j;
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+                        uint4& x = vr[k >> 1][2 * (k & 1) + j][c];
+                        if (full) {
+                            x = ldg16(src + j * RB + 8 * GG::VB * c);
+                        } else {
+                            x = make_uint4(0, 0, 0, 0);
+                            if (line != ~0u && tok >= lo && tok < t_end) x = ldg16(src + j * RB + 8 * GG::VB * c);
+                        }
+                    }
+                }
+            }
+        };
+
         int t0 = t_begin + warp * 16 * TG;
         uint32_t buf = 0;      // offset of the tile's buffer
         uint32_t lines = group_of(t0);
-        fetch(bufs, t0, lines);
+        if constexpr (DIRECT) {
+            load_k(t0, lines);
+            load_v(t0, lines);
+        } else {
+            fetch(bufs, t0, lines);
+        }
         lines = group_of(t0 + UNIT);
 
         // ---- queries as B fragments, in the order of the key pieces ---------------------------
@@ -509,10 +605,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
         }
 
         for (; t0 < t_end; t0 += UNIT) {
-            copies_wait<0>();
-            __syncwarp();
-            fetch(bufs + (GG::BUF - buf), t0 + UNIT, lines);
-            lines = group_of(t0 + 2 * UNIT);
+            const uint32_t lines_next = group_of(t0 + 2 * UNIT);
+            if constexpr (!DIRECT) {
+                copies_wait<0>();
+                __syncwarp();
+                fetch(bufs + (GG::BUF - buf), t0 + UNIT, lines);
+            }
             const uint32_t cur = bufs + buf;
             buf = GG::BUF - buf;
             // scores
@@ -525,8 +623,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
             for (int tg = 0; tg < TG; ++tg)
 #pragma unroll
                 for (int cc = 0; cc < KC; ++cc) {
-                    const uint32_t at = cur + 16 * tg * RB + (cc & 1 ? at_k1 : at_k0) + (cc >> 1) * 128;
-                    const uint4 k0 = lds16(at), k1 = lds16(at + 8 * RB);
+                    uint4 k0, k1;
+                    if constexpr (DIRECT) {
+                        k0 = kr[tg][0][cc];
+                        k1 = kr[tg][1][cc];
+                    } else {
+                        const uint32_t at = cur + 16 * tg * RB + (cc & 1 ? at_k1 : at_k0) + (cc >> 1) * 128;
+                        k0 = lds16(at);
+                        k1 = lds16(at + 8 * RB);
+                    }
                     const uint32_t r0[4] = {k0.x, k0.y, k0.z, k0.w};
                     const uint32_t r1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
@@ -548,7 +653,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
                 }
             float av[TG][2];      // log2 of the values' scales
             float top[NT][2], topw[NT][2];
-            const uint32_t have = lds4(cur + GG::OFF_L);
+            uint32_t have = live;
+            if constexpr (!DIRECT) have = lds4(cur + GG::OFF_L);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = topw[nt][0] = topw[nt][1] = -INFINITY;
 #pragma unroll
@@ -562,7 +668,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
                         kscale = __uint_as_float(w.x);
                         av[tg][hf] = lg2(__uint_as_float(w.y));
                     }
-                    const bool ok = have == kFull || (((have >> (2 * tg + hf)) & 1) && t0 + row >= lo && t0 + row < t_end);
+                    const bool ok = DIRECT ? (have >> (2 * tg + hf)) & 1
+                                           : have == kFull || (((have >> (2 * tg + hf)) & 1) && t0 + row >= lo && t0 + row < t_end);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -574,6 +681,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
                             if (KIND == FP8) topw[nt][i] = fmaxf(topw[nt][i], s + av[tg][hf]);
                         }
                 }
+            if constexpr (DIRECT) load_k(t0 + UNIT, lines);
             // raise the running maxima when a score passes them by more than kLazy
             bool up = false;
 #pragma unroll
@@ -659,8 +767,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
                     uint32_t v0[4], v1[4], v2[4], v3[4];
                     const uint32_t at = cur + 16 * tg * RB + c * 128;
                     if (VW == 4) {
-                        const uint4 x0 = lds16(at + at_v[0]), x1 = lds16(at + at_v[1]);
-                        const uint4 x2 = lds16(at + at_v[0] + 8 * RB), x3 = lds16(at + at_v[1] + 8 * RB);
+                        uint4 x0, x1, x2, x3;
+                        if constexpr (DIRECT) {
+                            x0 = vr[tg][0][c], x1 = vr[tg][1][c], x2 = vr[tg][2][c], x3 = vr[tg][3][c];
+                        } else {
+                            x0 = lds16(at + at_v[0]), x1 = lds16(at + at_v[1]);
+                            x2 = lds16(at + at_v[0] + 8 * RB), x3 = lds16(at + at_v[1] + 8 * RB);
+                        }
                         v0[0] = x0.x, v0[1] = x0.y, v0[2] = x0.z, v0[3] = x0.w;
                         v1[0] = x1.x, v1[1] = x1.y, v1[2] = x1.z, v1[3] = x1.w;
                         v2[0] = x2.x, v2[1] = x2.y, v2[2] = x2.z, v2[3] = x2.w;
@@ -696,6 +809,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
                         }
                     }
                 }
+            if constexpr (DIRECT) load_v(t0 + UNIT, lines);
+            lines = lines_next;
         }
 
         // ---- join the warps -----------------------------------------------------------------------
@@ -765,109 +880,118 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
 }
 
 constexpr int kJoinMost = 512;       // threads of a joining block, at most
-constexpr int kJoinPieces = 256;     // pieces weighed at a time
-
-// max over the block of two values (threads: a multiple of 32)
-__device__ __forceinline__ void block_max2(float& x, float& y, float2* sh) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
-    }
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(x, y);
-    __syncthreads();
-    for (int i = 0; i < (int)blockDim.x / 32; ++i) {
-        x = fmaxf(x, sh[i].x);
-        y = fmaxf(y, sh[i].y);
-    }
-}
 
 // Joins the pieces of one split stream for one head: piece 0 is record
-// `first`, piece j > 0 the first record of the j-th CTA after it.  The pieces
-// are weighed first (one round of loads over all of them), then summed by
-// groups of lanes with eight rows in flight each; a chain of rescaled sums
-// over one piece after the other took 121 us for 278 pieces.
+// `first`, piece j > 0 the first record of the j-th CTA after it.  A warp
+// takes 32 pieces at a time, a lane the maxima of one and D / 32 elements of
+// every row; the rows' loads go out before the weights are known.  Up to 8
+// pieces are one warp's work, without a barrier; more are dealt to all warps
+// of the block, whose sums meet in shared memory.  (One chain of rescaled sums
+// took 121 us for 278 pieces; with block-wide weights 16 sequences of 2K took
+// 5 us longer than this.)
 template <int D>
 __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__ AttendArgs a, int HP, bool fp8) {
-    constexpr int LPR = D / 4 < 32 ? D / 4 : 32;            // lanes of one record's row
-    constexpr int V4 = D / (4 * LPR);
-    __shared__ float so[kJoinMost / LPR][D];
-    __shared__ float wt[kJoinPieces];
-    __shared__ float2 sh[kJoinMost / 32];
-    __shared__ float sl[kJoinMost / 32];
+    constexpr int VE = D / 32, BATCH = 8;
+    __shared__ float so[kJoinMost / 32][D];
+    __shared__ float ss[kJoinMost / 32][3];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int4 ds = a.desc[blockIdx.x];
-    const int h = blockIdx.y;
+    const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (ds.z == 0 || h >= ds.y) return;
-    const int tid = threadIdx.x, grp = tid / LPR, ln = tid % LPR, groups = blockDim.x / LPR;
-    const int cta = ds.w >> 1;
-    auto record = [&](int j) { return (int64_t)(j == 0 ? ds.w : 2 * (cta + j)) * HP + h; };
-    float m = -INFINITY, M = -INFINITY, l = 0.f;            // l: this thread's share
-    float4 o[V4];
+    const bool alone = ds.z <= 8;
+    if (alone && warp > 0) return;
+    const int warps = alone ? 1 : blockDim.x >> 5;
+    const int cta = ds.w >> 1, mine = (ds.z - warp + warps - 1) / warps;
+    auto record = [&](int i) {
+        const int j = warp + i * warps;
+        return (int64_t)(j == 0 ? ds.w : 2 * (cta + j)) * HP + h;
+    };
+    struct alignas(4 * (VE < 4 ? VE : 4)) Row {
+        float v[VE];
+    };
+    float m = -INFINITY, M = -INFINITY, l = 0.f, o[VE];
 #pragma unroll
-    for (int v = 0; v < V4; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j0 = 0; j0 < ds.z; j0 += kJoinPieces) {
-        const int n = min(kJoinPieces, ds.z - j0);
-        float mn = m, Mn = M;
-        float4 s[kJoinPieces / 128];
+    for (int e = 0; e < VE; ++e) o[e] = 0.f;
+    for (int i0 = 0; i0 < mine; i0 += 32) {
+        const int n = min(32, mine - i0);
+        float4 s = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+        if (lane < n) s = a.rec_s[record(i0 + lane)];
+        Row r[BATCH];
+        auto load = [&](int i1) {
 #pragma unroll
-        for (int k = 0; k < kJoinPieces / 128; ++k) {
-            const int j = tid + k * blockDim.x;
-            s[k] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
-            if (j < n) s[k] = a.rec_s[record(j0 + j)];
-            mn = fmaxf(mn, s[k].x);
-            Mn = fmaxf(Mn, s[k].y);
+            for (int i = 0; i < BATCH; ++i)
+                if (i1 + i < n) r[i] = *reinterpret_cast<const Row*>(a.rec_o + record(i0 + i1 + i) * D + lane * VE);
+        };
+        load(0);
+        float mn = s.x, Mn = s.y;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) {
+            mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, k));
+            Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, k));
         }
-        block_max2(mn, Mn, sh);
-        l *= m == -INFINITY ? 1.f : ex2(m - mn);
+        mn = fmaxf(m, mn);
+        Mn = fmaxf(M, Mn);
+        const float fl = m == -INFINITY ? 1.f : ex2(m - mn), fo = M == -INFINITY ? 1.f : ex2(M - Mn);
+        l = l * fl + s.z * (s.x == -INFINITY ? 1.f : ex2(s.x - mn));
+        const float w = s.y == -INFINITY ? 1.f : ex2(s.y - Mn);
 #pragma unroll
-        for (int k = 0; k < kJoinPieces / 128; ++k) {
-            const int j = tid + k * blockDim.x;
-            if (j < n) wt[j] = s[k].y == -INFINITY ? 1.f : ex2(s[k].y - Mn);
-            l += s[k].z * (s[k].x == -INFINITY ? 1.f : ex2(s[k].x - mn));
-        }
-        __syncthreads();
-        const float f = M == -INFINITY ? 1.f : ex2(M - Mn);
+        for (int e = 0; e < VE; ++e) o[e] *= fo;
+        for (int i1 = 0; i1 < n; i1 += BATCH) {
+            if (i1) load(i1);
 #pragma unroll
-        for (int v = 0; v < V4; ++v) o[v] = make_float4(o[v].x * f, o[v].y * f, o[v].z * f, o[v].w * f);
-#pragma unroll 8
-        for (int j = grp; j < n; j += groups) {
-            const float w = wt[j];
-            const float* row = a.rec_o + record(j0 + j) * D;
+            for (int i = 0; i < BATCH; ++i) {
+                const float wi = __shfl_sync(0xffffffffu, w, i1 + i);
+                if (i1 + i < n) {
 #pragma unroll
-            for (int v = 0; v < V4; ++v) {
-                const float4 x = *reinterpret_cast<const float4*>(row + 4 * (ln + v * LPR));
-                o[v].x = fmaf(x.x, w, o[v].x);
-                o[v].y = fmaf(x.y, w, o[v].y);
-                o[v].z = fmaf(x.z, w, o[v].z);
-                o[v].w = fmaf(x.w, w, o[v].w);
+                    for (int e = 0; e < VE; ++e) o[e] = fmaf(r[i].v[e], wi, o[e]);
+                }
             }
         }
         m = mn;
         M = Mn;
-        __syncthreads();
     }
-#pragma unroll
-    for (int v = 0; v < V4; ++v) *reinterpret_cast<float4*>(&so[grp][4 * (ln + v * LPR)]) = o[v];
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
-    if ((tid & 31) == 0) sl[tid >> 5] = l;
-    __syncthreads();
-    float ll = 0.f;
-    for (int i = 0; i < (int)blockDim.x / 32; ++i) ll += sl[i];
-    const float f = (fp8 && M != -INFINITY && m != -INFINITY ? ex2(M - m) : 1.f) / ll;
-    for (int d = tid * 2; d < D; d += blockDim.x * 2) {
-        float y0 = 0.f, y1 = 0.f;
-        for (int w = 0; w < groups; ++w) {
-            y0 += so[w][d];
-            y1 += so[w][d + 1];
+    if (!alone) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) so[warp][lane * VE + e] = o[e];
+        if (lane == 0) {
+            ss[warp][0] = m;
+            ss[warp][1] = M;
+            ss[warp][2] = l;
         }
-        const int64_t at = (int64_t)(ds.x + h) * D + d;
-        *reinterpret_cast<uint32_t*>(a.out + at) = a.c.bf16 ? pack2<true>(y0 * f, y1 * f) : pack2<false>(y0 * f, y1 * f);
+        __syncthreads();
+        if (warp > 0) return;
+        float mm = -INFINITY, MM = -INFINITY, ll = 0.f;
+        for (int w = 0; w < warps; ++w) {
+            mm = fmaxf(mm, ss[w][0]);
+            MM = fmaxf(MM, ss[w][1]);
+        }
+#pragma unroll
+        for (int e = 0; e < VE; ++e) o[e] = 0.f;
+        for (int w = 0; w < warps; ++w) {
+            ll += ss[w][2] * (ss[w][0] == -INFINITY ? 1.f : ex2(ss[w][0] - mm));
+            const float x = ss[w][1] == -INFINITY ? 1.f : ex2(ss[w][1] - MM);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) o[e] = fmaf(so[w][lane * VE + e], x, o[e]);
+        }
+        m = mm;
+        M = MM;
+        l = ll;
     }
-    if (a.lse && tid == 0) a.lse[ds.x + h] = log_sum(m, ll);
+    const float f = (fp8 && M != -INFINITY && m != -INFINITY ? ex2(M - m) : 1.f) / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (int64_t)(ds.x + h) * D) + lane * (VE / 2);
+#pragma unroll
+    for (int e = 0; e < VE; e += 2)
+        dst[e / 2] = a.c.bf16 ? pack2<true>(o[e] * f, o[e + 1] * f) : pack2<false>(o[e] * f, o[e + 1] * f);
+    if (a.lse && lane == 0) a.lse[ds.x + h] = log_sum(m, l);
 }
+
+// Streams of up to so many units that all have an SM of their own stay whole:
+// no records, no second launch (2 kv heads of 64, us whole / split: 256 tokens
+// 4.3 / 7.1, 384 5.2 / 7.1, 512 7.0 / 7.3, 640 8.0 / 7.3, 1000 9.9 / 7.4)
+constexpr int kWholeUnits = 5;
 
 struct Plan {
     int nt, ht, unit, wave, waves, ctas, streams;
@@ -951,14 +1075,14 @@ int make_plan(const FkvPagedCache* c, int Hq, int pshift, Plan* p) {
                 FKV_ERR_UNSUPPORTED, "fkv_paged_attend: %lld streams of %lld tokens are too many",
                 (long long)streams, (long long)reach);
     p->streams = (int)streams;
-    const int per_sm = c->D * es == 512 ? 1 : c->D == 256 || p->nt == 2 ? 2 : 3;      // kPerSm
+    const int per_sm = c->D == 256 || p->nt == 2 ? 2 : 3;      // kPerSm
     const int ctas = per_sm * sm_count();
     const int64_t most = std::max<int64_t>(1, streams * std::max<int64_t>(units, 1));
-    p->wave = (int)std::min<int64_t>(ctas, most);
-    p->waves = most < (int64_t)ctas * kUnits2 ? 1 : most < (int64_t)ctas * kUnits3 ? 2 : 3;
+    p->split = units > kWholeUnits || (units > 1 && streams > sm_count());
+    p->wave = p->split ? (int)std::min<int64_t>(ctas, most) : std::max(p->streams, 1);
+    p->waves = !p->split || !c->fp8 || most < (int64_t)ctas * kUnits2 ? 1 : most < (int64_t)ctas * kUnits3 ? 2 : 3;
     p->ctas = p->wave * p->waves;
-    p->split = units > 1;
-    p->per_stream = p->streams <= p->ctas;
+    p->per_stream = p->split && p->streams <= p->ctas;
     const int hp = 8 * p->nt;
     const size_t recs = 2 * (size_t)p->ctas * hp;
     p->off_s = recs * c->D * sizeof(float);
@@ -1048,8 +1172,9 @@ extern "C" int fkv_paged_attend(const FkvPagedCache* c, int32_t Hq, float scale,
     FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
     if (!p.split) return FKV_OK;
     cfg.gridDim = dim3(p.per_stream ? p.streams : p.ctas, std::min(G, 8 * nt));
-    // many streams have few pieces each and fill the device with small blocks
-    cfg.blockDim = dim3((int64_t)cfg.gridDim.x * cfg.gridDim.y > 1024 ? 128 : kJoinMost);
+    // many streams have few pieces each; blocks for many would wait for room
+    // (16 sequences of 2K, 4 pieces a stream: 29.7 us with 512 threads, 25.6 with 128)
+    cfg.blockDim = dim3(p.ctas <= 8 * p.streams ? 128 : kJoinMost);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
     const bool fp8 = c->fp8 != 0;

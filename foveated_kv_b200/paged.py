@@ -23,7 +23,6 @@ Tensors shared by the three functions, P pages of ``page`` tokens:
 
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Sequence
 
 import torch
@@ -31,54 +30,12 @@ import torch
 from . import _native
 from .cache import FoveatedKVCache, compress_layer
 from .config import TierConfig
-from .rotary import check_frequencies, on_device, out16, refuse_grad, rows16
 
 _F16 = torch.float16
 _BF16 = torch.bfloat16
 _F8 = torch.float8_e4m3fn
 _I32 = torch.int32
 BAD_PAGE, BAD_POSITION = 1, 2
-
-
-def _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dtype):
-    """(descriptor of the checked pages, device index); dtype is that of the
-    tensors beside the pages."""
-    index, kind, shape = k_pages.get_device(), k_pages.dtype, k_pages.shape
-    if index < 0:
-        raise ValueError(f"{who}: pages must be CUDA tensors")
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not kind or v_pages.get_device() != index \
-            or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
-        raise ValueError(f"{who}: k_pages and v_pages must be contiguous (P, Hk, page, D) of one type and device")
-    if dtype is not _F16 and dtype is not _BF16:
-        raise ValueError(f"{who}: {dtype} beside the pages, expected float16 or bfloat16")
-    P, Hk, page, D = shape
-    if kind is _F8:
-        for s in (k_scale, v_scale):
-            if s is None or s.dtype is not torch.float32 or s.get_device() != index or s.shape != (P, Hk, page) \
-                    or not s.is_contiguous():
-                raise ValueError(f"{who}: float8 pages need contiguous float32 k_scale and v_scale (P, Hk, page)")
-        fp8, ks, vs = True, k_scale.data_ptr(), v_scale.data_ptr()
-    else:
-        if kind is not dtype:
-            raise ValueError(f"{who}: pages of {kind} beside {dtype}, expected the same type or float8_e4m3fn pages")
-        if k_scale is not None or v_scale is not None:
-            raise ValueError(f"{who}: scales go with float8 pages only")
-        fp8, ks, vs = False, None, None
-    ts, st = table.shape, table.stride()
-    if len(ts) != 2 or table.dtype is not _I32 or lens.dtype is not _I32 or table.get_device() != index \
-            or lens.get_device() != index or lens.shape != ts[:1] or not lens.is_contiguous():
-        raise ValueError(f"{who}: table must be int32 (B, W) and lens contiguous int32 (B,) on cuda:{index}")
-    B, W = ts
-    stride = st[0] if B > 1 else W
-    if (W > 1 and st[1] != 1) or stride < W:
-        raise ValueError(f"{who}: a row of table must be contiguous, and rows must not overlap")
-    word = None
-    if status is not None:
-        if status.dtype is not _I32 or status.get_device() != index or status.numel() != 1:
-            raise ValueError(f"{who}: status must be one int32 on cuda:{index}")
-        word = status.data_ptr()
-    return _native.PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, table.data_ptr(), lens.data_ptr(), word,
-                              B, Hk, D, page, P, W, stride, fp8, dtype is _BF16), index
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -103,52 +60,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     each row: scale = max(|row|, 2^-100) / 448, a row with an infinity or a NaN
     reads back as NaN.
     """
-    who = "paged_append"
-    dt, shape = k.dtype, k.shape
-    refuse_grad(who, k, v, q)
-    c, index = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dt)
-    nd, Hk, D = len(shape), k_pages.shape[1], k_pages.shape[3]
-    if v.shape != shape or nd not in (3, 4) or (nd == 4 and cu_new is not None) or shape[1] != Hk or shape[-1] != D:
-        raise ValueError(f"{who}: k {tuple(shape)} and v {tuple(v.shape)} must be (tokens, {Hk}, {D}), "
-                         f"or (B, {Hk}, n, {D}) without cu_new")
-    T, B, n, cu = shape[0], table.shape[0], 0, None
-    if cu_new is not None:
-        if cu_new.dtype is not _I32 or cu_new.get_device() != index or cu_new.shape != (B + 1,) \
-                or not cu_new.is_contiguous():
-            raise ValueError(f"{who}: cu_new must be contiguous int32 (B + 1,) on cuda:{index}")
-        cu = cu_new.data_ptr()
-    else:
-        if T != B:
-            raise ValueError(f"{who}: k holds {T} sequences, the table {B}")
-        n = shape[2] if nd == 4 else 1
-        T *= n
-    rot, freq = 0, None
-    if inv_freq is not None:
-        check_frequencies(who, inv_freq, index)
-        rot, freq = 2 * inv_freq.numel(), inv_freq.data_ptr()
-    k, k_st = rows16(who, "k", k, dt, index)
-    v, v_st = rows16(who, "v", v, dt, index)
-    Hq, q_ptr, qo_ptr, q_st, qo_st = 0, None, None, (0, 0, 0), (0, 0, 0)
-    if q is not None:
-        if inv_freq is None:
-            raise ValueError(f"{who}: q is only rotated; pass inv_freq with it")
-        if len(q.shape) != nd or q.shape[0] != shape[0] or q.shape[2:] != shape[2:]:
-            raise ValueError(f"{who}: q {tuple(q.shape)} does not go with k {tuple(shape)}")
-        Hq = q.shape[1]
-        q, q_st = rows16(who, "q", q, dt, index)
-        if q_out is None:
-            q_out, qo_st = rows16(who, "q_out", torch.empty_like(q), dt, index)
-        else:
-            q_out, qo_st = out16(who, "q_out", q_out, q, index)
-        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
-    elif q_out is not None:
-        raise ValueError(f"{who}: q_out without q")
-    if cu is None and nd == 3:               # one token per sequence: its row is the sequence's
-        k_st, v_st, q_st, qo_st = ((x[1], 0, x[2]) for x in (k_st, v_st, q_st, qo_st))
-    new = _native.PagedNew(T, n, Hq, rot, interleaved, amplitude, cu, freq, k.data_ptr(), v.data_ptr(), q_ptr, qo_ptr,
-                           *k_st, *v_st, *q_st, *qo_st)
-    _native.check(on_device(index, _native.load().fkv_paged_append, C.byref(c), C.byref(new)), "fkv_paged_append")
-    return q_out
+    return _native.ops().paged_append(k_pages, v_pages, table, lens, k_scale, v_scale, status, k, v, cu_new, q,
+                                      inv_freq, interleaved, amplitude, q_out)
 
 
 def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, max_len: int,
@@ -157,17 +70,7 @@ def paged_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor
     """The sequences' first max_len tokens as dense (k, v), each
     (B, Hk, max_len, D) of ``dtype`` (the pages' own type, or float16 for
     float8 pages), with zeros behind a sequence's end."""
-    who = "paged_read"
-    if dtype is None:
-        dtype = _F16 if k_pages.dtype is _F8 else k_pages.dtype
-    c, index = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dtype)
-    if max_len < 0:
-        raise ValueError(f"{who}: max_len {max_len}")
-    k = torch.empty((c.B, c.Hk, max_len, c.D), dtype=dtype, device=k_pages.device)
-    v = torch.empty_like(k)
-    _native.check(on_device(index, _native.load().fkv_paged_read, C.byref(c), max_len, k.data_ptr(), v.data_ptr()),
-                  "fkv_paged_read")
-    return k, v
+    return _native.ops().paged_read(k_pages, v_pages, table, lens, k_scale, v_scale, status, max_len, dtype)
 
 
 def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -184,39 +87,8 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     -inf.  Lengths are read on the device, so the call can be captured once and
     replayed as sequences grow within the table.
     """
-    who = "paged_attend"
-    dt, shape = q.dtype, q.shape
-    refuse_grad(who, q)
-    c, index = _cache(who, k_pages, v_pages, table, lens, k_scale, v_scale, status, dt)
-    B, Hk, D = table.shape[0], k_pages.shape[1], k_pages.shape[3]
-    if len(shape) not in (3, 4) or shape[0] != B or shape[-1] != D or shape[1] < 1 or shape[1] % Hk \
-            or (len(shape) == 4 and shape[2] != 1) or q.get_device() != index:
-        raise ValueError(f"{who}: q {tuple(shape)} must be (B, Hq, D) or (B, Hq, 1, D) on cuda:{index} with B {B}, "
-                         f"D {D} and Hq a multiple of {Hk}")
-    if window < 0:
-        raise ValueError(f"{who}: window {window}")
-    Hq = shape[1]
-    if not q.is_contiguous():
-        q = q.contiguous()
-    if q.data_ptr() & 15:
-        q = q.clone()
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != shape or out.dtype is not dt or out.get_device() != index or not out.is_contiguous() \
-            or out.data_ptr() & 15:
-        raise ValueError(f"{who}: out must be a contiguous, 16-byte aligned tensor like q")
-    lse = lse_ptr = ws_ptr = None
-    if return_lse:
-        lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device)
-        lse_ptr = lse.data_ptr()
-    lib, ref = _native.load(), C.byref(c)
-    nbytes = lib.fkv_paged_attend_workspace_bytes(ref, Hq)
-    if nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        ws_ptr = ws.data_ptr()
-    _native.check(on_device(index, lib.fkv_paged_attend, ref, Hq, D ** -0.5 if scale is None else scale, window,
-                            q.data_ptr(), out.data_ptr(), lse_ptr, ws_ptr, nbytes), "fkv_paged_attend")
-    return (out, lse) if return_lse else out
+    return _native.ops().paged_attend(k_pages, v_pages, table, lens, k_scale, v_scale, status, q, scale, window,
+                                      return_lse, out)
 
 
 class PagedKVCache:

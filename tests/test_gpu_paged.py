@@ -84,9 +84,8 @@ def test_attend_long_offsets():
     k[ids.long().cuda()] = p.k_pages[p.table[0, :4].long()]
     v[ids.long().cuda()] = p.v_pages[p.table[0, :4].long()]
     q = _rand(1, 32, D, dtype=F16)
-    want = fkv.paged_attend(q, **p.kw)
-    got = fkv.paged_attend(q, k, v, ids[None].cuda(), p.lens)
-    assert torch.equal(got, want)
+    got, lse = fkv.paged_attend(q, k, v, ids[None].cuda(), p.lens, return_lse=True)
+    R.check_attend(p, q, got, lse)
     new = _rand(1, Hk, D, dtype=F16, seed=3)
     fkv.paged_append(new, new, k, v, ids[None].cuda(), torch.tensor([page], dtype=torch.int32, device="cuda"))
     assert torch.equal(k[P - 1, :, page - 1], new[0])
