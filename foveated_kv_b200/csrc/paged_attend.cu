@@ -33,7 +33,7 @@
 // 8 kv heads, f16: 50.9 us, through shared memory 53.1; 33 ragged windows 46 /
 // 55).  8-bit pages need twice the instructions a byte, and registers could not
 // hide them: they go by 16-byte asynchronous copies through two buffers a warp
-// in shared memory (64 x 32K: 667 us direct, 505 through buffers).
+// in shared memory (64 x 32K: 531 us direct, 502 through buffers).
 //
 // 8-bit rows: codes become f16 exactly.  A key's scale multiplies its score.
 // A value's scale joins the exponent: w_n = exp2(x_n + log2 s_n - M) with a

@@ -22,7 +22,7 @@ using namespace fkvdev;
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
 constexpr float kRowFloor = 7.888609052210118e-31f;   // 2^-100
 
 struct AppendArgs {
@@ -92,7 +92,7 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, int t) {
     return p;
 }
 
-// A block takes up to 8 new tokens (or a slice of one's rows): D/8 lanes of a
+// A block takes up to 16 new tokens (or a slice of one's rows): D/8 lanes of a
 // warp to a row, first the tokens' 2 Hk key and value rows, then their Hq
 // query rows.
 template <int D, bool BF, bool FP8, bool IL, bool W16>
@@ -412,7 +412,7 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
     const int rows = kThreads / (c->D / 8);
     const int passes = (std::max(2 * c->Hk, n->Hq) + rows - 1) / rows;
     // few tokens: their rows are spread over more blocks
-    a.per_block = tokens_per_block(n->T);
+    a.per_block = tokens_per_block(n->T, 2 * c->Hk + n->Hq);
     a.by_kv = FastDiv(2 * (uint32_t)c->Hk);
     a.by_q = FastDiv((uint32_t)std::max(1, n->Hq));
     const dim3 grid((n->T + a.per_block - 1) / a.per_block, std::min(passes, std::max(1, 592 / n->T)));

@@ -10,7 +10,7 @@ using namespace fkvdev;
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 256;
 
 struct RotaryArgs {
     const uint16_t* q;
@@ -155,7 +155,7 @@ extern "C" int fkv_rotary(const FkvRotaryShape* sh, const uint16_t* q, const uin
     a.sign = sh->inverse ? -1.f : 1.f;
     const int rows = kThreads / (sh->D / 8);
     const int passes = (sh->Hq + sh->Hk + rows - 1) / rows;
-    a.per_block = tokens_per_block(tokens);
+    a.per_block = tokens_per_block(tokens, sh->Hq + sh->Hk);
     // rows of a block in the order of memory: (B, H, S, D) has a head's tokens together
     const int64_t* lead = sh->Hq ? a.qs : a.ks;
     a.tok_shift = -1;

@@ -42,7 +42,7 @@ __device__ __forceinline__ RotaryUnit rotary_unit(int u, int half, bool interlea
 }
 
 // x / n by a multiplication: exact while x * n < 2^32 (rows of a block: x is
-// under 8 tokens' rows)
+// under 16 tokens' rows)
 struct FastDiv {
     uint32_t n, m;
     FastDiv() = default;
@@ -50,11 +50,13 @@ struct FastDiv {
     __device__ __forceinline__ int div(int x) const { return n == 1 ? x : (int)__umulhi((uint32_t)x, m); }
 };
 
-// tokens of a block: as many as leave kMinBlocks blocks, a power of two
-constexpr int kMinBlocks = 148 * 16, kMostTokens = 8;
-inline int tokens_per_block(int64_t tokens) {
+// tokens of a block, a power of two: enough for some 300 rows, as long as that
+// leaves kMinBlocks blocks (16K tokens of 40 heads of 128, us with 4 / 8 / 16
+// tokens: 57.7 / 60.7 / 67; 32K tokens of 4 + 14 of 64: 40.5 with 8, 36 with 16)
+constexpr int kMinBlocks = 148 * 8, kMostTokens = 16, kBlockRows = 300;
+inline int tokens_per_block(int64_t tokens, int rows) {
     int p = 1;
-    while (p < kMostTokens && tokens / (2 * p) >= kMinBlocks) p *= 2;
+    while (p < kMostTokens && 2 * p * rows <= kBlockRows && tokens / (2 * p) >= kMinBlocks) p *= 2;
     return p;
 }
 
