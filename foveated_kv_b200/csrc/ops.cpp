@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -141,6 +142,14 @@ Rows new16(const Tensor& like) {
     }
     return r;
 }
+// An output that is `in` itself is written in place; any other overlap is a race.
+// (Views that interleave, as q and k of packed rows, cannot be told apart
+// cheaply and pass.)
+bool apart(const Tensor& out, const Tensor& in, bool same_is_fine) {
+    if (same_is_fine && out.data_ptr() == in.data_ptr() && out.strides() == in.strides()) return true;
+    const auto st = at::get_overlap_status(out, in);
+    return st != at::MemOverlapStatus::Full && st != at::MemOverlapStatus::Partial;
+}
 const double* frequencies(const char* who, const Tensor& f, int index) {
     require(f.scalar_type() == at::kDouble && f.dim() == 1 && index_of(f) == index && f.is_contiguous(), who,
             "inv_freq must be a contiguous float64 vector on cuda:", index);
@@ -200,6 +209,11 @@ PyObject* rotary(PyObject* const* args) {
         ki = rows16(who, "k", *k, dt, index);
         ko = k_out ? out16(who, "out", *k_out, *k, index) : new16(ki.t);
     }
+    if (q_out || k_out)
+        require((!q_out || (apart(qo.t, qi.t, true) && (!k || apart(qo.t, ki.t, false)))) &&
+                    (!k_out || (apart(ko.t, ki.t, true) && apart(ko.t, qi.t, false))) &&
+                    (!k || apart(qo.t, ko.t, false)),
+                who, "out overlaps an input that it is not");
     copy3(sh.q_stride, qi.st);
     copy3(sh.q_out_stride, qo.st);
     copy3(sh.k_stride, ki.st);
@@ -308,6 +322,8 @@ PyObject* append(PyObject* const* args) {
         n.interleaved = truth(args[12]);
         n.amplitude = (float)number(args[13]);
     }
+    require(p.c.n_pages == 0 || (p.c.k_pages != p.c.v_pages && (!p.c.fp8 || p.c.k_scale != p.c.v_scale)), who,
+            "k_pages and v_pages (and their scales) must be different tensors");
     require(q == nullptr || f != nullptr, who, "q is only rotated; pass inv_freq with it");
     require(q != nullptr || q_out == nullptr, who, "q_out without q");
     const c10::cuda::OptionalCUDAGuard guard(p.k->device());
@@ -320,6 +336,9 @@ PyObject* append(PyObject* const* args) {
         n.Hq = size32(q->size(1), who);
         qi = rows16(who, "q", *q, dt, p.index);
         qo = q_out ? out16(who, "q_out", *q_out, *q, p.index) : new16(qi.t);
+        if (q_out)
+            require(apart(qo.t, qi.t, true) && apart(qo.t, kr.t, false) && apart(qo.t, vr.t, false), who,
+                    "q_out overlaps an input that it is not");
         n.q = qi.ptr();
         n.q_out = qo.ptr();
     }
@@ -339,8 +358,7 @@ PyObject* append(PyObject* const* args) {
     return THPVariable_Wrap(qo.t);
 }
 
-// ---- paged_read(pages..., max_len, like) ----------------------------------------------------------
-// `like`: a 16-bit type as the element type's name, or None for the pages' own
+// ---- paged_read(pages..., max_len, dtype) ----------------------------------------------------------
 PyObject* read(PyObject* const* args) {
     const char* who = "paged_read";
     const Tensor& kp = tensor(args[0], who, "k_pages");
@@ -392,6 +410,7 @@ PyObject* attend(PyObject* const* args) {
         require(out.sizes() == q.sizes() && out.scalar_type() == dt && index_of(out) == p.index && out.is_contiguous() &&
                     (reinterpret_cast<uintptr_t>(out.data_ptr()) & 15) == 0,
                 who, "out must be a contiguous, 16-byte aligned tensor like q");
+        require(apart(out, q, false), who, "out overlaps q");
     }
     Tensor lse, ws;
     if (want_lse) lse = at::empty({p.c.B, Hq}, q.options().dtype(at::kFloat));

@@ -1102,7 +1102,7 @@ extern "C" size_t fkv_paged_attend_workspace_bytes(const FkvPagedCache* c, int32
     if (s.D != 64 && s.D != 128 && s.D != 256) return 0;
     if (s.page < 8 || s.page > 256 || (s.page & (s.page - 1)) || s.Hk < 1 || s.B < 0 || s.width < 0) return 0;
     while ((1 << pshift) < s.page) ++pshift;
-    if (Hq < 1 || Hq % s.Hk != 0 || ((int64_t)s.width << pshift) > INT_MAX) return 0;
+    if (Hq < 1 || Hq % s.Hk != 0 || ((int64_t)s.width << pshift) > 1 << 30) return 0;
     return make_plan(&s, Hq, pshift, &p) == FKV_OK ? p.bytes : 0;
 }
 
@@ -1139,6 +1139,10 @@ extern "C" int fkv_paged_attend(const FkvPagedCache* c, int32_t Hq, float scale,
                 "fkv_paged_attend: workspace not 16-byte aligned");
     AttendArgs a;
     a.c = *c;
+    if (c->n_pages == 0) {        // copies of no bytes still name an address
+        a.c.k_pages = a.c.v_pages = const_cast<uint16_t*>(q);
+        a.c.k_scale = a.c.v_scale = reinterpret_cast<float*>(const_cast<uint16_t*>(q));
+    }
     a.q = q;
     a.out = out;
     a.lse = lse;

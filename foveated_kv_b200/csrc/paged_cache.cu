@@ -345,7 +345,7 @@ int paged_check(const FkvPagedCache* c, const char* who, int* pshift) {
     int sh = 0;
     while ((1 << sh) < c->page) ++sh;
     *pshift = sh;
-    FKV_REQUIRE(((int64_t)c->width << sh) <= INT_MAX, FKV_ERR_UNSUPPORTED,
+    FKV_REQUIRE(((int64_t)c->width << sh) <= 1 << 30, FKV_ERR_UNSUPPORTED,
                 "%s: table reaches %lld tokens a sequence", who, (long long)c->width << sh);
     if (c->B == 0) return FKV_OK;
     FKV_REQUIRE(c->lens && (c->width == 0 || c->table) && (c->n_pages == 0 || (c->k_pages && c->v_pages)),

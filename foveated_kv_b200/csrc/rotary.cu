@@ -156,6 +156,7 @@ extern "C" int fkv_rotary(const FkvRotaryShape* sh, const uint16_t* q, const uin
     const int rows = kThreads / (sh->D / 8);
     const int passes = (sh->Hq + sh->Hk + rows - 1) / rows;
     a.per_block = tokens_per_block(tokens, sh->Hq + sh->Hk);
+    while ((size_t)a.per_block * a.half * 2 * sizeof(float) > (32u << 10)) a.per_block /= 2;   // at most 512 pairs
     // rows of a block in the order of memory: (B, H, S, D) has a head's tokens together
     const int64_t* lead = sh->Hq ? a.qs : a.ks;
     a.tok_shift = -1;

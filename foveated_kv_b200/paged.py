@@ -84,8 +84,12 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     default; ``window`` > 0 attends the last ``window`` tokens only.  Returns
     out, of q's shape, and with return_lse the natural log-sum-exp of the
     scaled scores, (B, Hq) float32.  A sequence without tokens gives zeros and
-    -inf.  Lengths are read on the device, so the call can be captured once and
-    replayed as sequences grow within the table.
+    -inf.  A score of +inf gives NaN and +inf; an infinite value gives a
+    non-finite output.  Lengths are read on the device, so the call can be
+    captured once and replayed as sequences grow within the table; neither they
+    nor the table may change while it runs.  The work split follows the table's
+    width and the lengths: the same inputs give the same bits, a wider table
+    may round differently.
     """
     return _native.ops().paged_attend(k_pages, v_pages, table, lens, k_scale, v_scale, status, q, scale, window,
                                       return_lse, out)
@@ -180,8 +184,13 @@ class PagedKVCache:
         self._step_lens.copy_(host[n:2 * n])
         self._cu.copy_(host[2 * n:])
 
+    def _check_slot(self, slot: int) -> None:
+        if not 0 <= slot < self.max_seqs:
+            raise ValueError(f"slot {slot} of {self.max_seqs}")
+
     def release(self, slot: int) -> None:
         """Empty a slot; its pages may be given to other sequences."""
+        self._check_slot(slot)
         self._free.extend(reversed(self._pages[slot]))
         self._pages[slot] = []
         self._lens[slot] = 0
@@ -211,6 +220,7 @@ class PagedKVCache:
 
     def read(self, layer: int, slot: int):
         """One sequence as dense keys and values (1, H_kv, length, D)."""
+        self._check_slot(slot)
         n = self._lens[slot]
         return paged_read(table=self.table[slot:slot + 1], lens=self.lens[slot:slot + 1], max_len=n,
                           dtype=self.dtype, status=self.status, **self.layers[layer])
@@ -219,6 +229,9 @@ class PagedKVCache:
                  keep_archive: bool = True) -> FoveatedKVCache:
         """Hand one sequence to the tiered cache: every layer read back and
         tiered by ``compress_layer``.  The slot keeps its pages."""
+        self._check_slot(slot)
+        if self._lens[slot] == 0:
+            raise ValueError(f"compress: slot {slot} is empty")
         fov = FoveatedKVCache(cfg)
         fov.layers = [compress_layer(*self.read(i, slot), fov.cfg,
                                      query[i] if isinstance(query, (list, tuple)) else query, keep_archive)

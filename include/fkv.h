@@ -353,7 +353,7 @@ typedef struct FkvPagedCache {
     int32_t B, Hk, D;            /* D: 64, 128 or 256 */
     int32_t page;                /* tokens of a page: a power of two from 8 to 256 */
     int32_t n_pages;
-    int32_t width;               /* table entries of a sequence */
+    int32_t width;               /* table entries of a sequence; width * page <= 2^30 */
     int32_t table_stride;        /* entries from one sequence's row to the next, >= width */
     int32_t fp8;
     int32_t bf16;                /* type of 16-bit pages and of every tensor beside them */
@@ -396,8 +396,9 @@ int fkv_paged_read(const FkvPagedCache* c, int32_t max_len, uint16_t* k, uint16_
 /* Attention of one token per sequence over its last `window` tokens (0: all):
  * q, out (B, Hq, D) 16-bit, 16-byte aligned; lse (B, Hq) f32 natural
  * log-sum-exp of the scaled scores, or NULL.  A sequence without tokens gives
- * zeros and -inf.  The workspace needs no initialisation; calls that share
- * one must not overlap on the GPU. */
+ * zeros and -inf.  table and lens must not change while the launch runs, and
+ * out must not overlap q.  The workspace needs no initialisation; calls that
+ * share one must not overlap on the GPU. */
 size_t fkv_paged_attend_workspace_bytes(const FkvPagedCache* c, int32_t Hq);
 int fkv_paged_attend(const FkvPagedCache* c, int32_t Hq, float scale, int32_t window,
                      const uint16_t* q, uint16_t* out, float* lse, void* workspace,

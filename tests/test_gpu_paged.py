@@ -168,6 +168,23 @@ def test_attend_nothing_to_do():
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+def test_a_pool_of_no_pages(fp8):
+    p = R.Pages(14, [0, 0], 2, 64, 16, F16, fp8, spare=0)
+    assert p.k_pages.shape[0] == 0
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q, k = _rand(2, 4, 64, dtype=F16), _rand(2, 2, 64, dtype=F16)
+    assert (fkv.paged_attend(q, status=st, **p.kw) == 0).all() and st.item() == 0
+    kw = dict(p.kw, lens=torch.tensor([20, 3], dtype=torch.int32, device="cuda"), table=p.table.abs())
+    fkv.paged_attend(q, status=st, **kw)
+    assert st.item() == 1
+    st.zero_()
+    fkv.paged_append(k, k, status=st, **kw)
+    assert st.item() == 1
+    dense = fkv.paged_read(max_len=20, **kw)
+    assert (dense[0] == 0).all() and (dense[1] == 0).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_attend_bad_pages_and_lengths(fp8):
     """A table entry that is no page leaves its tokens out; a length beyond the
     table is cut; the status word says so."""
@@ -592,6 +609,13 @@ def test_cache_limits_change_nothing():
     c.check()                                                    # reported once
     with pytest.raises(ValueError):
         PagedKVCache(1, 4, 2, 64, max_len=8).append(0, _rand(1, 2, 64, dtype=F16), _rand(1, 2, 64, dtype=F16))
+    for call in (lambda: c.release(2), lambda: c.read(0, -1), lambda: c.compress(5)):
+        with pytest.raises(ValueError):
+            call()
+    c.release(1)
+    with pytest.raises(ValueError):
+        c.compress(1)
+    assert c.read(0, 1)[0].shape == (1, 2, 0, 64)
     with pytest.raises(ValueError):
         PagedKVCache(1, 4, 2, 96, max_len=8)
     with pytest.raises(ValueError):
@@ -623,6 +647,9 @@ def test_refusals():
         lambda: W(k[:, :, None], k[:, :, None], cu_new=cu, **p.kw), lambda: W(k, k, inv_freq=f.float(), **p.kw),
         lambda: W(k, k, q=q, inv_freq=f, q_out=q[:, :1].expand(2, 4, 64), **p.kw),
         lambda: W(k.clone().requires_grad_(), k, **p.kw), lambda: W(k.bfloat16(), k.bfloat16(), **p.kw),
+        lambda: A(q, out=q, **p.kw), lambda: W(k, k, **dict(p.kw, v_pages=p.k_pages)),
+        lambda: W(k, k, **dict(e.kw, v_scale=e.k_scale)),
+        lambda: W(k, k.clone(), q=k.clone(), q_out=k, inv_freq=f, **p.kw),
         lambda: fkv.paged_read(max_len=-1, **p.kw), lambda: fkv.paged_read(max_len=4, dtype=BF16, **p.kw),
         lambda: fkv.paged_read(max_len=4, dtype=torch.float32, **e.kw),
     ]

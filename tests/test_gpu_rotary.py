@@ -102,6 +102,24 @@ def test_strides_views_and_alignment():
     assert torch.equal(fkv.apply_rotary(odd, None, step, f), fkv.apply_rotary(odd, None, pos, f))
 
 
+@pytest.mark.parametrize("H,D,rot,T", [(1, 1024, 1024, 20000), (1, 64, 64, 40000), (300, 64, 32, 5000), (8192, 8, 8, 3)])
+def test_many_tokens_or_heads(H, D, rot, T):
+    f, _ = fkv.rotary_frequencies(rot)
+    q, pos = _rand(T, H, D, dtype=torch.float16), torch.arange(T, device="cuda")
+    _check(q, fkv.apply_rotary(q, None, pos, f), pos, f)
+
+
+def test_overlapping_outputs_are_refused():
+    f, _ = fkv.rotary_frequencies(64)
+    buf, pos = _rand(11, 4, 64, dtype=torch.float16), torch.arange(10, device="cuda")
+    q, k = buf[:10], _rand(10, 4, 64, dtype=torch.float16, seed=1)
+    for out in ((buf[1:], k.clone()), (k, k.clone()), (q.clone(), q), (k, q)):
+        with pytest.raises(ValueError):
+            fkv.apply_rotary(q, k, pos, f, out=out)
+    with pytest.raises(ValueError):
+        fkv.apply_rotary(q, None, pos, f, out=buf[1:])
+
+
 def test_empty_and_passed_through_values():
     f, _ = fkv.rotary_frequencies(64)
     pos = torch.zeros(0, dtype=torch.int64, device="cuda")

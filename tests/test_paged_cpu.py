@@ -24,7 +24,7 @@ def _cache(**kw):
     (dict(D=96), -2), (dict(D=512), -2), (dict(page=24), -2), (dict(page=4), -2), (dict(page=512), -2),
     (dict(B=-1), -1), (dict(Hk=0), -1), (dict(n_pages=-1), -1), (dict(width=-1), -1), (dict(table_stride=3), -1),
     (dict(lens=None), -1), (dict(table=None), -1), (dict(k_pages=None), -1), (dict(fp8=1), -1),
-    (dict(k_pages=DUMMY + 8), -1), (dict(width=1 << 28, table_stride=1 << 28), -2),
+    (dict(k_pages=DUMMY + 8), -1), (dict(width=1 << 28, table_stride=1 << 28), -2), (dict(width=(1 << 26) + 1, table_stride=1 << 27), -2),
 ])
 def test_cache_descriptor_refusals(kw, rc):
     lib = _native.load()
