@@ -7,12 +7,13 @@
 //   without tokens gives zeros and a log-sum-exp of -inf.
 //
 // Work split.  A stream is one (sequence, kv head, tile of up to 8 NT query
-// heads); its tokens are cut into units of kUnit.  The units of all streams,
-// in order, are dealt to the CTAs of one wave in equal contiguous runs, so
-// every CTA reads the same number of bytes whatever the lengths are (the
-// lengths stay on the device: each CTA sums them up itself).  A CTA that
-// holds a whole stream writes its output; a piece of one is left as a record
-// (maximum, sum, unnormalised output) that a second, dependent launch joins.
+// heads); its tokens are cut into units of 64 or 128.  The units of all
+// streams, in order, are dealt to the CTAs of one wave in equal contiguous
+// runs (or falling ones, see Deal), so every CTA reads the same number of bytes
+// whatever the lengths are (the lengths stay on the device: each CTA sums them
+// up itself).  A CTA that holds a whole stream writes its output; a piece of
+// one is left as a record (maximum, sum, unnormalised output) that a second,
+// dependent launch joins.  Short streams that have an SM each stay whole.
 // No atomics and no counters: records and descriptors are written before they
 // are read in every call, so the workspace needs no initialisation, and two
 // calls share nothing.
@@ -157,6 +158,16 @@ struct Deal {
             const int share = waves == 2 ? 90 : k == 0 ? 80 : 13;
             r[k] = k >= waves ? 0 : k == waves - 1 ? (left + wave - 1) / wave : max(1, (int)((int64_t)each * share / 100));
             left = max(0, left - wave * r[k]);
+        }
+    }
+    // units [u0, u1) of a CTA
+    __device__ void range(int cta, int& u0, int& u1) const {
+        if (r[1] == 0) {
+            u0 = (int)min((int64_t)r[0] * cta, (int64_t)total);
+            u1 = min(u0 + r[0], total);
+        } else {
+            u0 = begin(cta);
+            u1 = begin(cta + 1);
         }
     }
     __device__ int begin(int cta) const {        // first unit of a CTA, at most `total`
@@ -319,18 +330,19 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
 
     // ---- this CTA's run of units ------------------------------------------------------------
     Deal deal;
-    int u0, u1;
+    int u0, u1, b = 0, prefix = 0;
     if (a.desc == nullptr) {               // a CTA per stream
         int lo, len;
-        const int b = blockIdx.x / HS;
+        b = blockIdx.x / HS;
         seq_range(a, b, lo, len);
         const int n = seq_units<UNIT>(lo, len);
         u0 = (blockIdx.x - b * HS) * n;
         u1 = u0 + n;
-        if (tid == 0) {
-            sh_b = b;
-            sh_prefix = 0;
-        }
+    } else if (B == 1) {                   // nothing to sum up
+        int lo, len;
+        seq_range(a, 0, lo, len);
+        deal = Deal(seq_units<UNIT>(lo, len) * HS, a.wave, a.waves);
+        deal.range(blockIdx.x, u0, u1);
     } else {
         const int per = (B + kThreads - 1) / kThreads;
         int mine = 0;
@@ -356,13 +368,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
         total *= HS;
         const int excl = before + incl - mine;
         deal = Deal(total, a.wave, a.waves);
-        if (a.waves == 1) {
-            u0 = min((int64_t)deal.r[0] * blockIdx.x, (int64_t)total);
-            u1 = min(u0 + deal.r[0], total);
-        } else {
-            u0 = deal.begin(blockIdx.x);
-            u1 = deal.begin(blockIdx.x + 1);
-        }
+        deal.range(blockIdx.x, u0, u1);
         if (u0 < u1 && u0 >= excl * HS && u0 < (excl + mine) * HS) {
             int b = tid * per, p = excl;
             while (b + 1 < B) {
@@ -391,8 +397,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
     }
     if (a.desc != nullptr && !a.per_stream && tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     if (u0 >= u1) return;
-    __syncthreads();
-    int b = sh_b, prefix = sh_prefix;
+    if (a.desc != nullptr && B > 1) {
+        __syncthreads();
+        b = sh_b;
+        prefix = sh_prefix;
+    }
 
     for (int u = u0; u < u1 && b < B;) {
         int lo, len;
@@ -990,8 +999,8 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
 
 // Streams of up to so many units that all have an SM of their own stay whole:
 // no records, no second launch (2 kv heads of 64, us whole / split: 256 tokens
-// 4.3 / 7.1, 384 5.2 / 7.1, 512 7.0 / 7.3, 640 8.0 / 7.3, 1000 9.9 / 7.4)
-constexpr int kWholeUnits = 5;
+// 5.2 / 6.6, 384 6.3 / 6.6, 512 7.2 / 6.6)
+constexpr int kWholeUnits = 4;
 
 struct Plan {
     int nt, ht, unit, wave, waves, ctas, streams;
