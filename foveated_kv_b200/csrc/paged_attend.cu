@@ -997,10 +997,15 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
     if (a.lse && lane == 0) a.lse[ds.x + h] = log_sum(m, l);
 }
 
-// Streams of up to so many units that all have an SM of their own stay whole:
-// no records, no second launch (2 kv heads of 64, us whole / split: 256 tokens
-// 5.2 / 6.6, 384 6.3 / 6.6, 512 7.2 / 6.6)
-constexpr int kWholeUnits = 4;
+// Streams of up to so many units stay whole, a CTA each: no records, no second
+// launch, and no CTA that starts on one short stream after another.  A few
+// streams (us whole / split, 2 kv heads of 64): 256 tokens 5.2 / 6.6, 384 6.3 /
+// 6.6, 512 7.2 / 6.6.  More streams than SMs (sequences of up to 500 tokens, 8
+// kv heads of 128, f16): 24 of them 13.7 / 15.7, 64 22.0 / 28.5 (all of 500:
+// 34.0 / 30.2), 128 34.8 / 48.0; up to 1000 tokens, 16 units: 64 35.5 / 37.3
+// (60.2 / 49.6).  Four waves of streams balance by themselves: 256 of up to
+// 1000 tokens 102 / 110.
+constexpr int kWholeFew = 4, kWholeUnits = 9, kWholeMany = 16;
 
 struct Plan {
     int nt, ht, unit, wave, waves, ctas, streams;
@@ -1087,7 +1092,7 @@ int make_plan(const FkvPagedCache* c, int Hq, int pshift, Plan* p) {
     const int per_sm = c->D == 256 || p->nt == 2 ? 2 : 3;      // kPerSm
     const int ctas = per_sm * sm_count();
     const int64_t most = std::max<int64_t>(1, streams * std::max<int64_t>(units, 1));
-    p->split = units > kWholeUnits || (units > 1 && streams > sm_count());
+    p->split = units > (streams >= 4 * (int64_t)ctas ? kWholeMany : streams > sm_count() ? kWholeUnits : kWholeFew);
     p->wave = p->split ? (int)std::min<int64_t>(ctas, most) : std::max(p->streams, 1);
     p->waves = !p->split || !c->fp8 || most < (int64_t)ctas * kUnits2 ? 1 : most < (int64_t)ctas * kUnits3 ? 2 : 3;
     p->ctas = p->wave * p->waves;
