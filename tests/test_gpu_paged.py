@@ -61,7 +61,9 @@ def test_attend_head_groups(Hq, Hk, D, fp8):
 @pytest.mark.parametrize("B,Hk,D,n,dtype,fp8", [
     (1, 1, 128, 20000, F16, False),      # one stream over the whole device
     (1, 2, 64, 70001, BF16, True),
-    (200, 4, 64, 300, F16, False),       # more streams than CTAs, several units each
+    (200, 4, 64, 300, F16, False),       # a CTA per stream, more streams than CTAs at once
+    (120, 4, 64, 1500, F16, False),      # more streams than CTAs, cut into units
+    (120, 4, 128, 1500, BF16, True),
     (64, 8, 64, 3100, F16, True),        # two waves of CTAs
     (48, 16, 64, 8000, BF16, True),      # three
 ])
