@@ -33,7 +33,6 @@ struct AppendArgs {
     const int32_t* cu_new;
     const double* inv_freq;
     int T, per_block, n_uniform, Hq, half, pshift;
-    FastDiv by_kv, by_q;                   // 2 Hk and Hq
     float amplitude;
 };
 
@@ -97,7 +96,7 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, int t) {
 // query rows.
 template <int D, bool BF, bool FP8, bool IL, bool W16>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
-    constexpr int LPR = D / 8, ROWS = kThreads / LPR, N = kRowsAtOnce;
+    constexpr int LPR = D / 8, ROWS = kThreads / LPR;
     extern __shared__ __align__(16) float turns[];       // cosines, sines: [per_block][half] each
     __shared__ Place places[kMostTokens];
     const int u = threadIdx.x % LPR, r = threadIdx.x / LPR;
@@ -114,42 +113,37 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
         }
         __syncthreads();
     }
+    // a thread stays with one token: its place and sines in registers, heads in
+    // steps.  All lanes of a warp take the same number of steps (the shuffles).
+    const int group = ROWS / a.per_block;                // rows of a token at a time
+    const int k = r % a.per_block, h0 = blockIdx.y * group + r / a.per_block, step = gridDim.y * group;
+    const bool mine = r < group * a.per_block && k < count;
+    const Place p = places[mine ? k : 0];
+    const bool live = mine && p.line >= 0;
     const RotaryUnit ru = rotary_unit(u, a.half, IL);
-    const int Hk = a.c.Hk, step = gridDim.y * ROWS;
-    const int kv = count * 2 * Hk;
-    for (int base = blockIdx.y * ROWS; base < kv; base += N * step) {
-        uint2 w[N][2];
-        int64_t line[N];
-        int tok[N];
-        bool isk[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int i = base + j * step + r;
-            const int k = a.by_kv.div(i), h = i - k * 2 * Hk;
-            w[j][0] = w[j][1] = make_uint2(0, 0);
-            line[j] = -1;
-            tok[j] = k;
-            isk[j] = h < Hk;
-            if (i < kv && places[k].line >= 0) {
-                const Place& p = places[k];
-                const int hh = isk[j] ? h : h - Hk;
-                line[j] = p.line + ((int64_t)hh << a.pshift);
-                load_unit<W16>(isk[j] ? a.k + p.k + hh * a.ks[2] : a.v + p.v + hh * a.vs[2], ru, w[j]);
-            }
+    float4 c = make_float4(0.f, 0.f, 0.f, 0.f), s = c;
+    if (ru.turned && live) {
+        c = *reinterpret_cast<const float4*>(cosines + k * a.half + 4 * u);
+        s = *reinterpret_cast<const float4*>(sines + k * a.half + 4 * u);
+    }
+    const int Hk = a.c.Hk;
+    for (int i = 0; i < Hk; i += step) {
+        const int h = i + h0;
+        const bool have = live && h < Hk;
+        uint2 w[2][2] = {};                              // the head's key and value
+        if (have) {
+            load_unit<W16>(a.k + p.k + h * a.ks[2], ru, w[0]);
+            load_unit<W16>(a.v + p.v + h * a.vs[2], ru, w[1]);
         }
+        const int64_t line = p.line + ((int64_t)h << a.pshift);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const bool turn = isk[j] && ru.turned && line[j] >= 0;
-            float4 c, s;
-            if (turn) {
-                c = *reinterpret_cast<const float4*>(cosines + tok[j] * a.half + 4 * u);
-                s = *reinterpret_cast<const float4*>(sines + tok[j] * a.half + 4 * u);
-            }
+        for (int j = 0; j < 2; ++j) {
+            void* pages = j == 0 ? a.c.k_pages : a.c.v_pages;
             if (FP8) {
                 float x[8];
                 unpack4<BF>(w[j][0], x);
                 unpack4<BF>(w[j][1], x + 4);
-                if (turn) rotary_apply(x, c, s, IL);
+                if (j == 0 && ru.turned) rotary_apply(x, c, s, IL);
                 // the largest magnitude by its bits: a NaN is above infinity and stays
                 uint32_t top = 0;
 #pragma unroll
@@ -158,55 +152,27 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
                 for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
                 float most = __uint_as_float(top);
                 most = most < kRowFloor ? kRowFloor : most;
-                if (line[j] >= 0) {
+                if (have) {
                     const float inv = 448.f / most;
                     const uint32_t lo = e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
                     const uint32_t hi = e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-                    uint8_t* dst = reinterpret_cast<uint8_t*>(isk[j] ? a.c.k_pages : a.c.v_pages) + line[j] * D;
+                    uint8_t* dst = reinterpret_cast<uint8_t*>(pages) + line * D;
                     if (W16) {
                         *reinterpret_cast<uint2*>(dst + ru.off0) = make_uint2(lo, hi);
                     } else {
                         *reinterpret_cast<uint32_t*>(dst + ru.off0) = lo;
                         *reinterpret_cast<uint32_t*>(dst + ru.off1) = hi;
                     }
-                    if (u == 0) (isk[j] ? a.c.k_scale : a.c.v_scale)[line[j]] = most / 448.f;
+                    if (u == 0) (j == 0 ? a.c.k_scale : a.c.v_scale)[line] = most / 448.f;
                 }
-            } else if (line[j] >= 0) {
-                if (turn) turn_unit<BF>(w[j], c, s, IL);
-                store_unit<W16>(reinterpret_cast<uint16_t*>(isk[j] ? a.c.k_pages : a.c.v_pages) + line[j] * D, ru, w[j]);
+            } else if (have) {
+                if (j == 0 && ru.turned) turn_unit<BF>(w[j], c, s, IL);
+                store_unit<W16>(reinterpret_cast<uint16_t*>(pages) + line * D, ru, w[j]);
             }
         }
     }
-    const int nq = count * a.Hq;
-    for (int i0 = blockIdx.y * ROWS + r; i0 < nq; i0 += N * step) {
-        uint2 w[N][2];
-        uint16_t* dst[N];
-        int tok[N];
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int i = i0 + j * step;
-            const int k = a.by_q.div(i), h = i - k * a.Hq;
-            w[j][0] = w[j][1] = make_uint2(0, 0);           // zeros where a token is not stored
-            dst[j] = nullptr;
-            tok[j] = -1;
-            if (i < nq) {
-                const Place& p = places[k];
-                dst[j] = a.q_out + p.q_out + h * a.qos[2];
-                if (p.line >= 0) {
-                    tok[j] = k;
-                    load_unit<W16>(a.q + p.q + h * a.qs[2], ru, w[j]);
-                }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            if (dst[j] == nullptr) continue;
-            if (ru.turned && tok[j] >= 0)
-                turn_unit<BF>(w[j], *reinterpret_cast<const float4*>(cosines + tok[j] * a.half + 4 * u),
-                              *reinterpret_cast<const float4*>(sines + tok[j] * a.half + 4 * u), IL);
-            store_unit<W16>(dst[j], ru, w[j]);
-        }
-    }
+    if (mine)                                            // zeros where a token is not stored
+        rotary_rows<BF, IL, W16>(a.q + p.q, a.qs[2], a.q_out + p.q_out, a.qos[2], h0, step, a.Hq, ru, c, s, live);
 }
 
 struct ReadArgs {
@@ -410,11 +376,9 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
     a.amplitude = n->amplitude;
     a.T = n->T;
     const int rows = kThreads / (c->D / 8);
-    const int passes = (std::max(2 * c->Hk, n->Hq) + rows - 1) / rows;
+    const int passes = (std::max(c->Hk, n->Hq) + rows - 1) / rows;
     // few tokens: their rows are spread over more blocks
-    a.per_block = tokens_per_block(n->T, 2 * c->Hk + n->Hq);
-    a.by_kv = FastDiv(2 * (uint32_t)c->Hk);
-    a.by_q = FastDiv((uint32_t)std::max(1, n->Hq));
+    a.per_block = std::min(tokens_per_block(n->T, 2 * c->Hk + n->Hq), rows);
     const dim3 grid((n->T + a.per_block - 1) / a.per_block, std::min(passes, std::max(1, 592 / n->T)));
     const size_t smem = (size_t)a.per_block * a.half * 2 * sizeof(float);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -22,8 +22,7 @@ struct RotaryArgs {
     int64_t ps[2];                          // strides of (batch, token)
     const double* inv_freq;
     int64_t tokens;
-    int S, Hq, Hk, D, half, per_block, tok_shift;   // tok_shift >= 0: tokens before heads
-    FastDiv by_heads;
+    int S, Hq, Hk, D, half, per_block;
     float amplitude;
     float sign;                             // of the sines: -1 turns back
 };
@@ -48,50 +47,22 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         sines[i] = sn * a.sign;
     }
     __syncthreads();
-    if (r >= rows) return;
+    // a thread stays with one token: its sines in registers, heads in steps
+    const int group = rows / a.per_block;                // rows of a token at a time
+    const int k = r % a.per_block, h = blockIdx.y * group + r / a.per_block;
+    if (r >= group * a.per_block || k >= n) return;
     const RotaryUnit ru = rotary_unit(u, a.half, IL);
-    const int H = a.Hq + a.Hk, total = n * H;
-    const int step = gridDim.y * rows;
-    // rows in the order of memory: heads of a token, or tokens of a head
-    for (int i0 = blockIdx.y * rows + r; i0 < (a.tok_shift >= 0 ? a.per_block * H : total); i0 += kRowsAtOnce * step) {
-        uint2 w[kRowsAtOnce][2];
-        uint16_t* dst[kRowsAtOnce];
-        int tok[kRowsAtOnce];
-#pragma unroll
-        for (int j = 0; j < kRowsAtOnce; ++j) {
-            const int i = i0 + j * step;
-            int k, h;
-            if (a.tok_shift >= 0) {
-                h = i >> a.tok_shift;
-                k = i & (a.per_block - 1);
-            } else {
-                k = a.by_heads.div(i);
-                h = i - k * H;
-            }
-            dst[j] = nullptr;
-            tok[j] = k;
-            if (k < n && h < H) {
-                const int64_t b = a.S == a.tokens ? 0 : (tok0 + k) / a.S, s = tok0 + k - b * a.S;
-                const uint16_t* src;
-                if (h < a.Hq) {
-                    src = a.q + b * a.qs[0] + s * a.qs[1] + h * a.qs[2];
-                    dst[j] = a.q_out + b * a.qos[0] + s * a.qos[1] + h * a.qos[2];
-                } else {
-                    src = a.k + b * a.ks[0] + s * a.ks[1] + (h - a.Hq) * a.ks[2];
-                    dst[j] = a.k_out + b * a.kos[0] + s * a.kos[1] + (h - a.Hq) * a.kos[2];
-                }
-                load_unit<W16>(src, ru, w[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < kRowsAtOnce; ++j) {
-            if (dst[j] == nullptr) continue;
-            if (ru.turned)
-                turn_unit<BF>(w[j], *reinterpret_cast<const float4*>(cosines + tok[j] * a.half + 4 * u),
-                              *reinterpret_cast<const float4*>(sines + tok[j] * a.half + 4 * u), IL);
-            store_unit<W16>(dst[j], ru, w[j]);
-        }
+    float4 c = make_float4(0.f, 0.f, 0.f, 0.f), sn = c;
+    if (ru.turned) {
+        c = *reinterpret_cast<const float4*>(cosines + k * a.half + 4 * u);
+        sn = *reinterpret_cast<const float4*>(sines + k * a.half + 4 * u);
     }
+    const int64_t b = a.S == a.tokens ? 0 : (tok0 + k) / a.S, s = tok0 + k - b * a.S;
+    const int step = gridDim.y * group;
+    rotary_rows<BF, IL, W16>(a.q + b * a.qs[0] + s * a.qs[1], a.qs[2], a.q_out + b * a.qos[0] + s * a.qos[1], a.qos[2], h,
+                             step, a.Hq, ru, c, sn, true);
+    rotary_rows<BF, IL, W16>(a.k + b * a.ks[0] + s * a.ks[1], a.ks[2], a.k_out + b * a.kos[0] + s * a.kos[1], a.kos[2], h,
+                             step, a.Hk, ru, c, sn, true);
 }
 
 }  // namespace
@@ -154,15 +125,10 @@ extern "C" int fkv_rotary(const FkvRotaryShape* sh, const uint16_t* q, const uin
     a.amplitude = sh->amplitude;
     a.sign = sh->inverse ? -1.f : 1.f;
     const int rows = kThreads / (sh->D / 8);
-    const int passes = (sh->Hq + sh->Hk + rows - 1) / rows;
+    const int passes = (std::max(sh->Hq, sh->Hk) + rows - 1) / rows;
     a.per_block = tokens_per_block(tokens, sh->Hq + sh->Hk);
-    while ((size_t)a.per_block * a.half * 2 * sizeof(float) > (32u << 10)) a.per_block /= 2;   // at most 512 pairs
-    // rows of a block in the order of memory: (B, H, S, D) has a head's tokens together
-    const int64_t* lead = sh->Hq ? a.qs : a.ks;
-    a.tok_shift = -1;
-    if (a.per_block > 1 && lead[1] < lead[2])
-        for (a.tok_shift = 0; (1 << a.tok_shift) < a.per_block;) ++a.tok_shift;
-    a.by_heads = FastDiv((uint32_t)(sh->Hq + sh->Hk));
+    // at most 512 pairs, and a row of each token at a time
+    while ((size_t)a.per_block * a.half * 2 * sizeof(float) > (32u << 10) || a.per_block > rows) a.per_block /= 2;
     // few tokens: their heads are spread over more blocks
     const int gy = (int)std::min<int64_t>(passes, std::max<int64_t>(1, 592 / tokens));
     const dim3 grid((unsigned)((tokens + a.per_block - 1) / a.per_block), (unsigned)gy);

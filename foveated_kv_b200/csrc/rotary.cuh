@@ -41,19 +41,10 @@ __device__ __forceinline__ RotaryUnit rotary_unit(int u, int half, bool interlea
     return r;
 }
 
-// x / n by a multiplication: exact while x * n < 2^32 (rows of a block: x is
-// under 16 tokens' rows)
-struct FastDiv {
-    uint32_t n, m;
-    FastDiv() = default;
-    __host__ explicit FastDiv(uint32_t n_) : n(n_), m((uint32_t)((0x100000000ull + n_ - 1) / n_)) {}
-    __device__ __forceinline__ int div(int x) const { return n == 1 ? x : (int)__umulhi((uint32_t)x, m); }
-};
-
-// tokens of a block, a power of two: enough for some 300 rows, as long as that
-// leaves kMinBlocks blocks (16K tokens of 40 heads of 128, us with 4 / 8 / 16
-// tokens: 57.7 / 60.7 / 67; 32K tokens of 4 + 14 of 64: 40.5 with 8, 36 with 16)
-constexpr int kMinBlocks = 148 * 8, kMostTokens = 16, kBlockRows = 300;
+// tokens of a block, a power of two: enough for some 450 rows, as long as that
+// leaves kMinBlocks blocks (us with 4 / 8 / 16 tokens: 16K tokens of 40 heads of
+// 128 57.9 / 55.5 / -, 28.7K of 4 + 4 + 28, fp8 - / 83.8 / 86.1)
+constexpr int kMinBlocks = 148 * 8, kMostTokens = 16, kBlockRows = 450;
 inline int tokens_per_block(int64_t tokens, int rows) {
     int p = 1;
     while (p < kMostTokens && 2 * p * rows <= kBlockRows && tokens / (2 * p) >= kMinBlocks) p *= 2;
@@ -62,7 +53,7 @@ inline int tokens_per_block(int64_t tokens, int rows) {
 
 // rows that a thread has in flight: loads come first, since the compiler may
 // not move them over the stores of rows that could be the same memory
-constexpr int kRowsAtOnce = 2;
+constexpr int kRowsAtOnce = 4;
 
 // cosine and sine (times amplitude) of pair p at position pos
 __device__ __forceinline__ void rotary_pair(const double* __restrict__ inv_freq, int p, int64_t pos,
@@ -152,6 +143,33 @@ __device__ __forceinline__ void turn_unit(uint2 (&w)[2], const float4 c, const f
     rotary_apply(x, c, s, interleaved);
     w[0] = pack4<BF>(x);
     w[1] = pack4<BF>(x + 4);
+}
+
+// Rows of one token, heads h, h + step, ...: turned or passed through, or zeros
+// where !live
+template <bool BF, bool IL, bool W16>
+__device__ __forceinline__ void rotary_rows(const uint16_t* src, int64_t src_head, uint16_t* dst, int64_t dst_head,
+                                            int h, int step, int heads, const RotaryUnit& ru, const float4 c,
+                                            const float4 s, bool live) {
+    src += h * src_head;
+    dst += h * dst_head;
+    const int64_t ds = step * src_head, dd = step * dst_head;
+    for (; h < heads; h += kRowsAtOnce * step) {
+        uint2 w[kRowsAtOnce][2];
+#pragma unroll
+        for (int j = 0; j < kRowsAtOnce; ++j) {
+            w[j][0] = w[j][1] = make_uint2(0, 0);
+            if (live && h + j * step < heads) load_unit<W16>(src + j * ds, ru, w[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kRowsAtOnce; ++j) {
+            if (h + j * step >= heads) break;
+            if (ru.turned && live) turn_unit<BF>(w[j], c, s, IL);
+            store_unit<W16>(dst + j * dd, ru, w[j]);
+        }
+        src += kRowsAtOnce * ds;
+        dst += kRowsAtOnce * dd;
+    }
 }
 
 }  // namespace fkvdev
