@@ -9,7 +9,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 
 def build(verbose: bool = False, jobs: int = 8) -> str:
     csrc = os.path.join(HERE, "csrc")
-    cmd = ["make", "-C", csrc, f"-j{jobs}"]
+    cmd = ["make", "-C", csrc, f"-j{jobs}", f"PY={sys.executable}"]
     res = subprocess.run(cmd, capture_output=not verbose, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"libfkv build failed:\n{res.stdout}\n{res.stderr}")

@@ -93,9 +93,10 @@ __device__ __forceinline__ float log_sum(float m, float l) {
     return m == INFINITY ? m : (m + log2f(l)) * 0.6931471805599453f;
 }
 
+// (not .nc: an early launch's data may be written while the grid already waits)
 __device__ __forceinline__ uint4 ldg16(const void* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
