@@ -131,11 +131,12 @@ class PagedKVCache:
         self.layers = [dict(k_pages=new(), v_pages=new(), k_scale=scale(), v_scale=scale()) for _ in range(n_layers)]
         self.width = -(-max_len // page)
         self.table = torch.full((max_seqs, self.width), -1, dtype=_I32, device=device)
-        self.lens = torch.zeros(max_seqs, dtype=_I32, device=device)
+        # lengths; lengths of the slots with a new token in this step, else 0; the
+        # counts' prefix sums
+        self._state = torch.zeros(3 * max_seqs + 1, dtype=_I32, device=device)
+        self.lens, self._step_lens, self._cu = self._state.split([max_seqs, max_seqs, max_seqs + 1])
         self.status = torch.zeros(1, dtype=_I32, device=device)
         self.device = self.table.device
-        self._step_lens = torch.zeros(max_seqs, dtype=_I32, device=device)   # 0: no new token in this step
-        self._cu = torch.zeros(max_seqs + 1, dtype=_I32, device=device)
         self._packed = None                                                   # None: no step begun
         self._new_rows = 0
         self._lens = [0] * max_seqs
@@ -170,7 +171,7 @@ class PagedKVCache:
                 ids.append(self._free.pop())
                 self._pages[s].append(ids[-1])
         if at:
-            upd = torch.tensor([at, ids], dtype=torch.int64).to(self.device)
+            upd = self._send([at, ids], torch.int64)
             self.table.view(-1)[upd[0]] = upd[1].to(_I32)
         self._lens = lens
         self._packed = max(counts) > 1
@@ -178,11 +179,11 @@ class PagedKVCache:
         cu = [0]
         for c in counts:
             cu.append(cu[-1] + c)
-        host = torch.tensor(lens + [n if c else 0 for n, c in zip(lens, counts)] + cu, dtype=_I32).to(self.device)
-        n = self.max_seqs
-        self.lens.copy_(host[:n])
-        self._step_lens.copy_(host[n:2 * n])
-        self._cu.copy_(host[2 * n:])
+        self._state.copy_(self._send(lens + [n if c else 0 for n, c in zip(lens, counts)] + cu, _I32))
+
+    def _send(self, values, dtype) -> torch.Tensor:
+        """Host values on the device, without waiting for the stream."""
+        return torch.tensor(values, dtype=dtype, pin_memory=True).to(self.device, non_blocking=True)
 
     def _check_slot(self, slot: int) -> None:
         if not 0 <= slot < self.max_seqs:
