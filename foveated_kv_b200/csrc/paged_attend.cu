@@ -6,7 +6,7 @@
 //   n over the last `window` (or all) tokens of the sequence; a sequence
 //   without tokens gives zeros and a log-sum-exp of -inf.
 //
-// Work split.  A stream is one (sequence, kv head, tile of up to 8 NT query
+// Work split.  A stream is one (sequence, kv head, group of up to 16 query
 // heads); its tokens are cut into units of 64 or 128.  The units of all
 // streams, in order, are dealt to the CTAs of one wave in equal contiguous
 // runs (or falling ones, see Deal), so every CTA reads the same number of bytes
@@ -68,8 +68,8 @@ struct AttendArgs {
     const uint16_t* q;
     uint16_t* out;
     float* lse;
-    float* rec_o;      // (2 per CTA, 8 NT heads, D)
-    float4* rec_s;     // (2 per CTA, 8 NT heads): m, M, l
+    float* rec_o;      // (2 per CTA, HP heads, D)
+    float4* rec_s;     // (2 per CTA, HP heads): m, M, l
     int4* desc;        // first output row, heads, pieces (0: nothing to join), first record
     int Hq, G, HT, pshift, window, per_stream, wave, waves;
     float sl2;         // scale * log2(e)
@@ -268,8 +268,8 @@ __device__ __forceinline__ void sts4(uint32_t a, uint32_t v) {
 }
 
 // CTAs per SM that a kernel's registers are held to
-template <int D, int NT, int KIND>
-constexpr int kPerSm = D == 256 || NT == 2 ? 2 : 3;
+template <int D, int HP>
+constexpr int kPerSm = D == 256 || HP == 16 ? 2 : 3;
 
 // Units of work of sequence b: tokens [lo, len), cut from lo rounded down to 16.
 __device__ __forceinline__ void seq_range(const AttendArgs& a, int b, int& lo, int& len) {
@@ -288,27 +288,31 @@ __device__ __forceinline__ int seq_units(int lo, int len) {
 }
 
 // the warps' results of one piece of a stream; shares its memory with the buffers
-template <int D, int NT>
+template <int D, int HP>
 struct Join {
-    float o[kWarps][8 * NT][D + 2];
-    float m[kWarps][8 * NT], M[kWarps][8 * NT], l[kWarps][8 * NT];
+    float o[kWarps][HP][D + 2];
+    float m[kWarps][HP], M[kWarps][HP], l[kWarps][HP];
 };
 
-template <int D, int NT, int KIND>
+template <int D, int HP, int KIND>
 constexpr size_t smem_bytes() {
     const size_t r = Geo<D, KIND>::DIRECT ? 0 : (size_t)kWarps * Geo<D, KIND>::BUFS * Geo<D, KIND>::BUF;
-    return r > sizeof(Join<D, NT>) ? r : sizeof(Join<D, NT>);
+    return r > sizeof(Join<D, HP>) ? r : sizeof(Join<D, HP>);
 }
 
-template <int D, int NT, int KIND>
-__global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(const __grid_constant__ AttendArgs a) {
+// HP query heads a CTA, in NT tiles of 8 columns: 8 a tile, or, of up to 4, one
+// in every other column, so that a lane has one head's scores and not the
+// scores of one that does not exist beside them (16 x 1K f16, 4 heads a group:
+// 17.7 -> 16.9 us).
+template <int D, int HP, int KIND>
+__global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const __grid_constant__ AttendArgs a) {
     using GG = Geo<D, KIND>;
     constexpr int TG = GG::TG, UNIT = GG::UNIT, KC = GG::KC, KS = GG::KS, VC = GG::VC, VW = GG::VW, MT = GG::MT;
     constexpr int RB = GG::RB;
     constexpr bool DIRECT = GG::DIRECT;
-    constexpr int HP = 8 * NT;
+    constexpr int NT = HP == 16 ? 2 : 1, NI = HP == 4 ? 1 : 2;   // tiles; heads of a lane in one
     extern __shared__ __align__(128) unsigned char smem_raw[];
-    Join<D, NT>& sm = *reinterpret_cast<Join<D, NT>*>(smem_raw);
+    Join<D, HP>& sm = *reinterpret_cast<Join<D, HP>*>(smem_raw);
     __shared__ int sh_scan[kWarps], sh_b, sh_prefix;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int B = a.c.B, HS = a.c.Hk * a.HT;
@@ -431,7 +435,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
             for (int i = 0; i < QW; ++i) {
                 qw[nt][i] = make_uint4(0, 0, 0, 0);
                 const int at = (t + 4 * (i / (KS / 2))) * GG::KE + 8 * (i % (KS / 2));
-                if (nt * 8 + g < nh) qw[nt][i] = ldg16(a.q + (row0 + nt * 8 + g) * D + at);
+                const int h = HP == 4 ? g >> 1 : nt * 8 + g;
+                if ((HP != 4 || (g & 1) == 0) && h < nh) qw[nt][i] = ldg16(a.q + (row0 + h) * D + at);
             }
 
         // row of the 8-token group `lane` of the tile at token t0 (~0: nothing to read)
@@ -683,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
+                        for (int i = 0; i < NI; ++i) {
                             float& s = x[tg][nt][2 * hf + i];
                             s *= KIND == FP8 ? qs[nt][i] * kscale : qs[nt][i];
                             if (!ok) s = -INFINITY;
@@ -697,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < NI; ++i) {
                     up |= top[nt][i] > m[nt][i] + kLazy;
                     if (KIND == FP8) up |= topw[nt][i] > M[nt][i] + kLazy;
                 }
@@ -705,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
+                    for (int i = 0; i < NI; ++i) {
                         float y = top[nt][i], z = topw[nt][i];
 #pragma unroll
                         for (int s = 4; s < 32; s <<= 1) {
@@ -749,13 +754,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
                         const float x0 = x[tg][nt][2 * hf], x1 = x[tg][nt][2 * hf + 1];
-                        const float p0 = ex2(x0 - m0), p1 = ex2(x1 - m1);
+                        const float p0 = ex2(x0 - m0), p1 = NI == 2 ? ex2(x1 - m1) : 0.f;
                         l[nt][0] += p0;
-                        l[nt][1] += p1;
+                        if (NI == 2) l[nt][1] += p1;
                         float w0 = p0, w1 = p1;
                         if (KIND == FP8) {
                             w0 = ex2(x0 + av[tg][hf] - M0);
-                            w1 = ex2(x1 + av[tg][hf] - M1);
+                            if (NI == 2) w1 = ex2(x1 + av[tg][hf] - M1);
                         }
                         if (KIND == FP8) {
                             pf[tg][nt][hf] = transpose8x8(pack2<false>(w0, w1));
@@ -829,20 +834,21 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, NT, KIND>) attend_kernel(c
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < NI; ++i) {
+                const int h = HP == 4 ? t : nt * 8 + 2 * t + i;
                 float s = l[nt][i];
 #pragma unroll
                 for (int k = 4; k < 32; k <<= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
                 if (g == 0) {
-                    sm.m[warp][nt * 8 + 2 * t + i] = m[nt][i];
-                    sm.M[warp][nt * 8 + 2 * t + i] = KIND == FP8 ? M[nt][i] : m[nt][i];
-                    sm.l[warp][nt * 8 + 2 * t + i] = s;
+                    sm.m[warp][h] = m[nt][i];
+                    sm.M[warp][h] = KIND == FP8 ? M[nt][i] : m[nt][i];
+                    sm.l[warp][h] = s;
                 }
 #pragma unroll
                 for (int k = 0; k < MT; ++k) {
                     // row tile k covers elements d, d + 1 of this lane's piece
                     const int d = (k / (GG::VE / 2)) * 8 * GG::VE + g * GG::VE + 2 * (k % (GG::VE / 2));
-                    *reinterpret_cast<float2*>(&sm.o[warp][nt * 8 + 2 * t + i][d]) = make_float2(o[nt][k][i], o[nt][k][2 + i]);
+                    *reinterpret_cast<float2*>(&sm.o[warp][h][d]) = make_float2(o[nt][k][i], o[nt][k][2 + i]);
                 }
             }
         __syncthreads();
@@ -1009,35 +1015,33 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
 constexpr int kWholeFew = 4, kWholeUnits = 9, kWholeMany = 16;
 
 struct Plan {
-    int nt, ht, unit, wave, waves, ctas, streams;
+    int hp, ht, unit, wave, waves, ctas, streams;
     bool split, per_stream;
     size_t bytes, off_s, off_d;
 };
 
 using Kernel = void (*)(const AttendArgs);
 
-template <int D, int NT, int KIND>
+template <int D, int HP, int KIND>
 void entry(Kernel& k, size_t& smem) {
-    k = attend_kernel<D, NT, KIND>;
-    smem = smem_bytes<D, NT, KIND>();
+    k = attend_kernel<D, HP, KIND>;
+    smem = smem_bytes<D, HP, KIND>();
+}
+
+template <int D, int HP>
+void entry_h(int kind, Kernel& k, size_t& smem) {
+    switch (kind) {
+        case F16: entry<D, HP, F16>(k, smem); break;
+        case BF16: entry<D, HP, BF16>(k, smem); break;
+        default: entry<D, HP, FP8>(k, smem); break;
+    }
 }
 
 template <int D>
-void entry_d(int nt, int kind, Kernel& k, size_t& smem) {
-    if constexpr (D == 256) {           // 16 heads' accumulators do not fit the registers
-        switch (kind) {
-            case F16: entry<D, 1, F16>(k, smem); break;
-            case BF16: entry<D, 1, BF16>(k, smem); break;
-            default: entry<D, 1, FP8>(k, smem); break;
-        }
-    } else switch (nt * 4 + kind) {
-        case 4: entry<D, 1, F16>(k, smem); break;
-        case 5: entry<D, 1, BF16>(k, smem); break;
-        case 6: entry<D, 1, FP8>(k, smem); break;
-        case 8: entry<D, 2, F16>(k, smem); break;
-        case 9: entry<D, 2, BF16>(k, smem); break;
-        default: entry<D, 2, FP8>(k, smem); break;
-    }
+void entry_d(int hp, int kind, Kernel& k, size_t& smem) {
+    if (hp == 4) entry_h<D, 4>(kind, k, smem);
+    else if (hp == 8) entry_h<D, 8>(kind, k, smem);
+    else if constexpr (D != 256) entry_h<D, 16>(kind, k, smem);
 }
 
 int kind_of(const FkvPagedCache* c) { return c->fp8 ? FP8 : c->bf16 ? BF16 : F16; }
@@ -1074,13 +1078,14 @@ int raise_smem(Kernel k, size_t smem) {
     return FKV_OK;
 }
 
-// 8-head tiles that one warp takes together
-int tiles_of(int G, int D) { return G <= 8 || D == 256 ? 1 : 2; }
+// query heads of a group that a CTA takes together (16 heads' accumulators of 256
+// do not fit the registers)
+int heads_of(int G, int D) { return G <= 4 ? 4 : G <= 8 || D == 256 ? 8 : 16; }
 
 int make_plan(const FkvPagedCache* c, int Hq, int pshift, Plan* p) {
     const int G = Hq / c->Hk;
-    p->nt = tiles_of(G, c->D);
-    p->ht = (G + 8 * p->nt - 1) / (8 * p->nt);
+    p->hp = heads_of(G, c->D);
+    p->ht = (G + p->hp - 1) / p->hp;
     const int es = c->fp8 ? 1 : 2;
     p->unit = kWarps * 16 * (c->D * es >= 256 ? 1 : 2);      // Geo::UNIT
     const int64_t reach = (int64_t)c->width << pshift;
@@ -1090,7 +1095,7 @@ int make_plan(const FkvPagedCache* c, int Hq, int pshift, Plan* p) {
                 FKV_ERR_UNSUPPORTED, "fkv_paged_attend: %lld streams of %lld tokens are too many",
                 (long long)streams, (long long)reach);
     p->streams = (int)streams;
-    const int per_sm = c->D == 256 || p->nt == 2 ? 2 : 3;      // kPerSm
+    const int per_sm = c->D == 256 || p->hp == 16 ? 2 : 3;      // kPerSm
     const int ctas = per_sm * sm_count();
     const int64_t most = std::max<int64_t>(1, streams * std::max<int64_t>(units, 1));
     p->split = units > (streams >= 4 * (int64_t)ctas ? kWholeMany : streams > sm_count() ? kWholeUnits : kWholeFew);
@@ -1098,8 +1103,7 @@ int make_plan(const FkvPagedCache* c, int Hq, int pshift, Plan* p) {
     p->waves = !p->split || !c->fp8 || most < (int64_t)ctas * kUnits2 ? 1 : most < (int64_t)ctas * kUnits3 ? 2 : 3;
     p->ctas = p->wave * p->waves;
     p->per_stream = p->split && p->streams <= p->ctas;
-    const int hp = 8 * p->nt;
-    const size_t recs = 2 * (size_t)p->ctas * hp;
+    const size_t recs = 2 * (size_t)p->ctas * p->hp;
     p->off_s = recs * c->D * sizeof(float);
     p->off_d = p->off_s + recs * sizeof(float4);
     p->bytes = p->split ? p->off_d + (size_t)std::max(p->ctas, 1) * sizeof(int4) : 0;
@@ -1134,12 +1138,12 @@ extern "C" int fkv_paged_attend(const FkvPagedCache* c, int32_t Hq, float scale,
     FKV_REQUIRE(q && out, FKV_ERR_INVALID, "fkv_paged_attend: NULL pointer");
     FKV_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0, FKV_ERR_INVALID,
                 "fkv_paged_attend: q / out not 16-byte aligned");
-    const int G = Hq / c->Hk, nt = tiles_of(G, c->D);
-    Kernel k;
-    size_t smem;
-    if (c->D == 64) entry_d<64>(nt, kind_of(c), k, smem);
-    else if (c->D == 128) entry_d<128>(nt, kind_of(c), k, smem);
-    else entry_d<256>(nt, kind_of(c), k, smem);
+    const int G = Hq / c->Hk, hp = heads_of(G, c->D);
+    Kernel k = nullptr;
+    size_t smem = 0;
+    if (c->D == 64) entry_d<64>(hp, kind_of(c), k, smem);
+    else if (c->D == 128) entry_d<128>(hp, kind_of(c), k, smem);
+    else entry_d<256>(hp, kind_of(c), k, smem);
     // a row's number is kept in 32 bits (2^32 rows of 64 bytes are more than the device holds)
     FKV_REQUIRE(((int64_t)c->n_pages * c->Hk << pshift) < 0xFFFFFFFFll, FKV_ERR_UNSUPPORTED,
                 "fkv_paged_attend: %d pages of %d x %d rows are too many", c->n_pages, c->Hk, c->page);
@@ -1190,15 +1194,15 @@ extern "C" int fkv_paged_attend(const FkvPagedCache* c, int32_t Hq, float scale,
     cfg.numAttrs = p.ctas <= sm_count() ? 1 : 0;
     FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
     if (!p.split) return FKV_OK;
-    cfg.gridDim = dim3(p.per_stream ? p.streams : p.ctas, std::min(G, 8 * nt));
+    cfg.gridDim = dim3(p.per_stream ? p.streams : p.ctas, std::min(G, hp));
     // many streams have few pieces each; blocks for many would wait for room
     // (16 sequences of 2K, 4 pieces a stream: 29.7 us with 512 threads, 25.6 with 128)
     cfg.blockDim = dim3(p.ctas <= 8 * p.streams ? 128 : kJoinMost);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
     const bool fp8 = c->fp8 != 0;
-    if (c->D == 64) FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<64>, a, 8 * nt, fp8));
-    else if (c->D == 128) FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<128>, a, 8 * nt, fp8));
-    else FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<256>, a, 8 * nt, fp8));
+    if (c->D == 64) FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<64>, a, hp, fp8));
+    else if (c->D == 128) FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<128>, a, hp, fp8));
+    else FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<256>, a, hp, fp8));
     return FKV_OK;
 }
