@@ -317,9 +317,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int B = a.c.B, HS = a.c.Hk * a.HT;
     const bool bf = KIND == BF16 || (KIND == FP8 && a.c.bf16);
-    // launched while its predecessor drains; nothing is read before this
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    await_predecessor();
     // this lane's places in a buffer: fragment rows g of K, rows 2t and 2t + 1 of V
     const uint32_t bufs = smem_u32(smem_raw) + warp * (GG::BUFS * GG::BUF);
     const int tok_k = DIRECT ? g : token_of<RB>(g);
@@ -910,8 +908,7 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
     constexpr int VE = D / 32, BATCH = 8;
     __shared__ float so[kJoinMost / 32][D];
     __shared__ float ss[kJoinMost / 32][3];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    await_predecessor();
     const int4 ds = a.desc[blockIdx.x];
     const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (ds.z == 0 || h >= ds.y) return;
@@ -1179,30 +1176,18 @@ extern "C" int fkv_paged_attend(const FkvPagedCache* c, int32_t Hq, float scale,
     a.waves = p.waves;
     a.sl2 = scale * 1.4426950408889634f;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.ctas);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cfg.attrs = at;
     // launched early only where the grid leaves room beside its predecessor:
     // 8.4 -> 7.3 us for 1K tokens, but 508 -> 526 for 64 x 32K, whose CTAs then
     // settled unevenly beside the last joining blocks
-    cfg.numAttrs = p.ctas <= sm_count() ? 1 : 0;
-    FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, a));
+    FKV_CUDA_CHECK(fkv::launch_beside(k, dim3(p.ctas), kThreads, smem, s, p.ctas <= sm_count(), a));
     if (!p.split) return FKV_OK;
-    cfg.gridDim = dim3(p.per_stream ? p.streams : p.ctas, std::min(G, hp));
+    const dim3 grid(p.per_stream ? p.streams : p.ctas, std::min(G, hp));
     // many streams have few pieces each; blocks for many would wait for room
     // (16 sequences of 2K, 4 pieces a stream: 29.7 us with 512 threads, 25.6 with 128)
-    cfg.blockDim = dim3(p.ctas <= 8 * p.streams ? 128 : kJoinMost);
-    cfg.dynamicSmemBytes = 0;
-    cfg.numAttrs = 1;
+    const int threads = p.ctas <= 8 * p.streams ? 128 : kJoinMost;
     const bool fp8 = c->fp8 != 0;
-    if (c->D == 64) FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<64>, a, hp, fp8));
-    else if (c->D == 128) FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<128>, a, hp, fp8));
-    else FKV_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<256>, a, hp, fp8));
+    FKV_CUDA_CHECK(c->D == 64    ? fkv::launch_beside(join_kernel<64>, grid, threads, 0, s, true, a, hp, fp8)
+                   : c->D == 128 ? fkv::launch_beside(join_kernel<128>, grid, threads, 0, s, true, a, hp, fp8)
+                                 : fkv::launch_beside(join_kernel<256>, grid, threads, 0, s, true, a, hp, fp8));
     return FKV_OK;
 }

@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     __shared__ Place places[kMostTokens];
     const int u = threadIdx.x % LPR, r = threadIdx.x / LPR;
     const int tok0 = blockIdx.x * a.per_block, count = min(a.per_block, a.T - tok0);
+    await_predecessor();
     if (threadIdx.x < count) places[threadIdx.x] = place_of(a, tok0 + threadIdx.x);
     __syncthreads();
     float* cosines = turns;
@@ -266,21 +267,20 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
 }
 
 template <int D, bool BF, bool FP8>
-void launch_append(const AppendArgs& a, dim3 grid, size_t smem, bool il, bool wide, cudaStream_t s) {
-    if (wide) append_kernel<D, BF, FP8, true, true><<<grid, kThreads, smem, s>>>(a);
-    else if (il) append_kernel<D, BF, FP8, true, false><<<grid, kThreads, smem, s>>>(a);
-    else append_kernel<D, BF, FP8, false, false><<<grid, kThreads, smem, s>>>(a);
+cudaError_t launch_append(const AppendArgs& a, dim3 grid, size_t smem, bool il, bool wide, cudaStream_t s) {
+    const bool early = (int64_t)grid.x * grid.y <= kEarlyBlocks;
+    if (wide) return fkv::launch_beside(append_kernel<D, BF, FP8, true, true>, grid, kThreads, smem, s, early, a);
+    if (il) return fkv::launch_beside(append_kernel<D, BF, FP8, true, false>, grid, kThreads, smem, s, early, a);
+    return fkv::launch_beside(append_kernel<D, BF, FP8, false, false>, grid, kThreads, smem, s, early, a);
 }
 
 template <int D>
-void launch_append(const AppendArgs& a, dim3 grid, size_t smem, bool il, bool wide, cudaStream_t s) {
-    if (a.c.bf16) {
-        if (a.c.fp8) launch_append<D, true, true>(a, grid, smem, il, wide, s);
-        else launch_append<D, true, false>(a, grid, smem, il, wide, s);
-    } else {
-        if (a.c.fp8) launch_append<D, false, true>(a, grid, smem, il, wide, s);
-        else launch_append<D, false, false>(a, grid, smem, il, wide, s);
-    }
+cudaError_t launch_append(const AppendArgs& a, dim3 grid, size_t smem, bool il, bool wide, cudaStream_t s) {
+    if (a.c.bf16)
+        return a.c.fp8 ? launch_append<D, true, true>(a, grid, smem, il, wide, s)
+                       : launch_append<D, true, false>(a, grid, smem, il, wide, s);
+    return a.c.fp8 ? launch_append<D, false, true>(a, grid, smem, il, wide, s)
+                   : launch_append<D, false, false>(a, grid, smem, il, wide, s);
 }
 
 template <int D>
@@ -383,10 +383,9 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
     const size_t smem = (size_t)a.per_block * a.half * 2 * sizeof(float);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool il = n->interleaved != 0;
-    if (c->D == 64) launch_append<64>(a, grid, smem, il, wide, s);
-    else if (c->D == 128) launch_append<128>(a, grid, smem, il, wide, s);
-    else launch_append<256>(a, grid, smem, il, wide, s);
-    FKV_LAUNCH_CHECK();
+    FKV_CUDA_CHECK(c->D == 64    ? launch_append<64>(a, grid, smem, il, wide, s)
+                   : c->D == 128 ? launch_append<128>(a, grid, smem, il, wide, s)
+                                 : launch_append<256>(a, grid, smem, il, wide, s));
     return FKV_OK;
 }
 

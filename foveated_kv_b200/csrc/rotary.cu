@@ -4,6 +4,7 @@
 #include <climits>
 
 #include "fkv_common.h"
+#include "paged.cuh"
 #include "rotary.cuh"
 
 using namespace fkvdev;
@@ -36,6 +37,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     const int n = (int)min((int64_t)a.per_block, a.tokens - tok0);
     float* cosines = turns;
     float* sines = turns + a.per_block * a.half;
+    await_predecessor();
     for (int i = threadIdx.x; i < n * a.half; i += kThreads) {
         const int k = i / a.half;
         const int64_t b = (tok0 + k) / a.S, s = tok0 + k - b * a.S, at = b * a.ps[0] + s * a.ps[1];
@@ -135,14 +137,19 @@ extern "C" int fkv_rotary(const FkvRotaryShape* sh, const uint16_t* q, const uin
     const size_t smem = (size_t)a.per_block * a.half * 2 * sizeof(float);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool p64 = sh->pos64 != 0;
+    const bool early = (int64_t)grid.x * grid.y <= kEarlyBlocks;
+    auto run = [&](void (*k)(RotaryArgs, bool)) {
+        return fkv::launch_beside(k, grid, kThreads, smem, s, early, a, p64);
+    };
+    cudaError_t e;
     switch ((sh->bf16 ? 4 : 0) | (sh->interleaved ? 2 : 0) | (wide ? 1 : 0)) {
-        case 0: rotary_kernel<false, false, false><<<grid, kThreads, smem, s>>>(a, p64); break;
-        case 2: rotary_kernel<false, true, false><<<grid, kThreads, smem, s>>>(a, p64); break;
-        case 3: rotary_kernel<false, true, true><<<grid, kThreads, smem, s>>>(a, p64); break;
-        case 4: rotary_kernel<true, false, false><<<grid, kThreads, smem, s>>>(a, p64); break;
-        case 6: rotary_kernel<true, true, false><<<grid, kThreads, smem, s>>>(a, p64); break;
-        default: rotary_kernel<true, true, true><<<grid, kThreads, smem, s>>>(a, p64); break;
+        case 0: e = run(rotary_kernel<false, false, false>); break;
+        case 2: e = run(rotary_kernel<false, true, false>); break;
+        case 3: e = run(rotary_kernel<false, true, true>); break;
+        case 4: e = run(rotary_kernel<true, false, false>); break;
+        case 6: e = run(rotary_kernel<true, true, false>); break;
+        default: e = run(rotary_kernel<true, true, true>); break;
     }
-    FKV_LAUNCH_CHECK();
+    FKV_CUDA_CHECK(e);
     return FKV_OK;
 }

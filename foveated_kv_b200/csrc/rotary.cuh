@@ -51,6 +51,9 @@ inline int tokens_per_block(int64_t tokens, int rows) {
     return p;
 }
 
+// grids of up to so many blocks are launched beside their predecessor
+constexpr int kEarlyBlocks = 148 * 4;
+
 // rows that a thread has in flight: loads come first, since the compiler may
 // not move them over the stores of rows that could be the same memory
 constexpr int kRowsAtOnce = 4;
