@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -134,12 +135,18 @@ Rows out16(const char* who, const char* name, const Tensor& t, const Tensor& lik
     require(ok, who, name, " must be 8-byte aligned rows that do not overlap, with strides of a multiple of 4 elements");
     return r;
 }
+// an output, straight from the CUDA allocator (through the dispatcher a call
+// with two outputs took a microsecond longer)
+Tensor make(at::IntArrayRef sizes, at::ScalarType dt, const at::Device& dev) {
+    return at::detail::empty_cuda(sizes, dt, dev, std::nullopt);
+}
+// an output of t's shape: in t's order of memory if that is dense
 Rows new16(const Tensor& like) {
-    Rows r{at::empty_like(like), {}};
-    if (!addressable(r.t, r.st)) {
-        r.t = at::empty(like.sizes(), like.options());
-        addressable(r.t, r.st);
-    }
+    Rows r{like.is_non_overlapping_and_dense()
+               ? at::detail::empty_strided_cuda(like.sizes(), like.strides(), like.scalar_type(), like.device())
+               : make(like.sizes(), like.scalar_type(), like.device()),
+           {}};
+    addressable(r.t, r.st);
     return r;
 }
 // An output that is `in` itself is written in place; any other overlap is a race.
@@ -370,9 +377,8 @@ PyObject* read(PyObject* const* args) {
     }
     const Pages p = pages(who, args, dt);
     const c10::cuda::OptionalCUDAGuard guard(kp.device());
-    const auto opt = kp.options().dtype(dt);
     const int64_t shape[4] = {p.c.B, p.c.Hk, max_len, p.c.D};
-    const Tensor k = at::empty(shape, opt), v = at::empty(shape, opt);
+    const Tensor k = make(shape, dt, kp.device()), v = make(shape, dt, kp.device());
     check(p_read(&p.c, max_len, static_cast<uint16_t*>(k.data_ptr()), static_cast<uint16_t*>(v.data_ptr()),
                  c10::cuda::getCurrentCUDAStream(p.index).stream()),
           "fkv_paged_read");
@@ -404,7 +410,7 @@ PyObject* attend(PyObject* const* args) {
     if (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) q = q.clone();
     Tensor out;
     if (out0 == nullptr) {
-        out = at::empty(q.sizes(), q.options());
+        out = make(q.sizes(), dt, q.device());
     } else {
         out = *out0;
         require(out.sizes() == q.sizes() && out.scalar_type() == dt && index_of(out) == p.index && out.is_contiguous() &&
@@ -413,9 +419,9 @@ PyObject* attend(PyObject* const* args) {
         require(apart(out, q, false), who, "out overlaps q");
     }
     Tensor lse, ws;
-    if (want_lse) lse = at::empty({p.c.B, Hq}, q.options().dtype(at::kFloat));
+    if (want_lse) lse = make({p.c.B, Hq}, at::kFloat, q.device());
     const size_t bytes = p_attend_ws(&p.c, Hq);
-    if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    if (bytes) ws = make({(int64_t)bytes}, at::kByte, q.device());
     check(p_attend(&p.c, Hq, (float)scale, window, static_cast<const uint16_t*>(q.data_ptr()),
                    static_cast<uint16_t*>(out.data_ptr()), want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr,
                    bytes ? ws.data_ptr() : nullptr, bytes, c10::cuda::getCurrentCUDAStream(p.index).stream()),
