@@ -674,3 +674,32 @@ def test_other_device():
     want = fkv.paged_attend(q, **p.kw)
     kw = {k: None if v is None else v.to("cuda:1") for k, v in p.kw.items()}
     assert torch.equal(fkv.paged_attend(q.to("cuda:1"), **kw).to("cuda:0"), want)
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are captured (kernels load and workspaces are made there)."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, foveated_kv_b200 as fkv
+kp, vp = (torch.randn(20, 2, 16, 128, device="cuda").bfloat16() for _ in range(2))
+table = torch.arange(20, dtype=torch.int32, device="cuda").view(1, 20)
+lens = torch.tensor([300], dtype=torch.int32, device="cuda")
+q, k = (torch.randn(1, h, 128, device="cuda").bfloat16() for h in (8, 2))
+f = fkv.rotary_frequencies(128)[0]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    qr = fkv.paged_append(k, k, kp, vp, table, lens, q=q, inv_freq=f)
+    o = fkv.paged_attend(qr, kp, vp, table, lens)
+    r = fkv.apply_rotary(q, None, lens - 1, f)
+    d = fkv.paged_read(kp, vp, table, lens, 300)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(r, qr)
+assert torch.equal(o, fkv.paged_attend(qr, kp, vp, table, lens))
+assert torch.equal(d[1][0, :, 299], k[0])
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=root)
