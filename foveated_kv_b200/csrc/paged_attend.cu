@@ -883,7 +883,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
         }
         if (a.desc && chunk == 0 && tid == 0) {
             // the CTA that holds a stream's first unit says how to join it
-            const int pieces = whole ? 0 : deal.cta_of(s_end - 1) - (int)blockIdx.x + 1;
+            // (never past the last CTA's records, even if a length grew under way)
+            const int pieces = whole ? 0 : min(deal.cta_of(s_end - 1), (int)gridDim.x - 1) - (int)blockIdx.x + 1;
             const int4 d = make_int4((int)row0, nh, pieces, slot);
             if (a.per_stream) a.desc[b * HS + stream] = d;
             else if (!whole) a.desc[blockIdx.x] = d;
