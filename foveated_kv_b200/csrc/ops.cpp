@@ -124,6 +124,10 @@ Rows rows16(const char* who, const char* name, const Tensor& t, at::ScalarType d
     }
     return r;
 }
+// A graph of autograd that saved a tensor written here must notice.
+void written(const Tensor* t) {
+    if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 // the same of a tensor that is written: it must be so already
 Rows out16(const char* who, const char* name, const Tensor& t, const Tensor& like, int index) {
     require(t.sizes() == like.sizes() && t.scalar_type() == like.scalar_type() && index_of(t) == index, who, name,
@@ -178,7 +182,7 @@ PyObject* rotary(PyObject* const* args) {
     const auto dt = q.scalar_type();
     require(index >= 0, who, "q must be a CUDA tensor");
     require(is16(dt), who, "q is ", dt, ", expected float16 or bfloat16");
-    refuse_grad(who, {&q, k});
+    refuse_grad(who, {&q, k, q_out, k_out});
     const int64_t nd = q.dim();
     require(nd == 3 || nd == 4, who, "q must be (B, H, S, D) or (T, H, D), got ", q.sizes());
     FkvRotaryShape sh = {};
@@ -228,6 +232,8 @@ PyObject* rotary(PyObject* const* args) {
     check(p_rotary(&sh, qi.ptr(), k ? ki.ptr() : nullptr, pos.data_ptr(), freq, qo.ptr(), k ? ko.ptr() : nullptr,
                    c10::cuda::getCurrentCUDAStream(index).stream()),
           "fkv_rotary");
+    written(q_out);
+    written(k_out);
     if (k == nullptr) return THPVariable_Wrap(qo.t);
     PyObject* r = PyTuple_New(2);
     PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(qo.t));
@@ -238,7 +244,7 @@ PyObject* rotary(PyObject* const* args) {
 // ---- the pages: k_pages, v_pages, table, lens, k_scale, v_scale, status -------------------------
 struct Pages {
     FkvPagedCache c = {};
-    const Tensor* k;
+    const Tensor *k, *v, *k_scale, *v_scale;
     int index;
 };
 Pages pages(const char* who, PyObject* const* args, at::ScalarType dt) {
@@ -247,7 +253,11 @@ Pages pages(const char* who, PyObject* const* args, at::ScalarType dt) {
     const Tensor &table = tensor(args[2], who, "table"), &lens = tensor(args[3], who, "lens");
     const Tensor *ks = maybe(args[4], who, "k_scale"), *vs = maybe(args[5], who, "v_scale");
     const Tensor* status = maybe(args[6], who, "status");
+    refuse_grad(who, {&k, &v, ks, vs});
     p.k = &k;
+    p.v = &v;
+    p.k_scale = ks;
+    p.v_scale = vs;
     const int index = p.index = index_of(k);
     const auto kind = k.scalar_type();
     require(index >= 0, who, "pages must be CUDA tensors");
@@ -302,7 +312,7 @@ PyObject* append(PyObject* const* args) {
     const Tensor &k = tensor(args[7], who, "k"), &v = tensor(args[8], who, "v");
     const Tensor *cu = maybe(args[9], who, "cu_new"), *q = maybe(args[10], who, "q");
     const Tensor *f = maybe(args[11], who, "inv_freq"), *q_out = maybe(args[14], who, "q_out");
-    refuse_grad(who, {&k, &v, q});
+    refuse_grad(who, {&k, &v, q, q_out});
     const auto dt = k.scalar_type();
     const Pages p = pages(who, args, dt);
     const int64_t nd = k.dim();
@@ -344,8 +354,9 @@ PyObject* append(PyObject* const* args) {
         qi = rows16(who, "q", *q, dt, p.index);
         qo = q_out ? out16(who, "q_out", *q_out, *q, p.index) : new16(qi.t);
         if (q_out)
-            require(apart(qo.t, qi.t, true) && apart(qo.t, kr.t, false) && apart(qo.t, vr.t, false), who,
-                    "q_out overlaps an input that it is not");
+            require(apart(qo.t, qi.t, true) && apart(qo.t, kr.t, false) && apart(qo.t, vr.t, false) &&
+                        apart(qo.t, *p.k, false) && apart(qo.t, *p.v, false),
+                    who, "q_out overlaps an input that it is not");
         n.q = qi.ptr();
         n.q_out = qo.ptr();
     }
@@ -361,6 +372,7 @@ PyObject* append(PyObject* const* args) {
             s[1] = 0;
         }
     check(p_append(&p.c, &n, c10::cuda::getCurrentCUDAStream(p.index).stream()), "fkv_paged_append");
+    for (const Tensor* t : {p.k, p.v, p.k_scale, p.v_scale, q_out}) written(t);
     if (q == nullptr) Py_RETURN_NONE;
     return THPVariable_Wrap(qo.t);
 }
@@ -393,7 +405,7 @@ PyObject* attend(PyObject* const* args) {
     const char* who = "paged_attend";
     const Tensor& q0 = tensor(args[7], who, "q");
     const Tensor* out0 = maybe(args[11], who, "out");
-    refuse_grad(who, {&q0});
+    refuse_grad(who, {&q0, out0});
     const auto dt = q0.scalar_type();
     const Pages p = pages(who, args, dt);
     const int64_t nd = q0.dim();
@@ -416,7 +428,8 @@ PyObject* attend(PyObject* const* args) {
         require(out.sizes() == q.sizes() && out.scalar_type() == dt && index_of(out) == p.index && out.is_contiguous() &&
                     (reinterpret_cast<uintptr_t>(out.data_ptr()) & 15) == 0,
                 who, "out must be a contiguous, 16-byte aligned tensor like q");
-        require(apart(out, q, false), who, "out overlaps q");
+        require(apart(out, q, false) && apart(out, *p.k, false) && apart(out, *p.v, false), who,
+                "out overlaps an input");
     }
     Tensor lse, ws;
     if (want_lse) lse = make({p.c.B, Hq}, at::kFloat, q.device());
@@ -426,6 +439,7 @@ PyObject* attend(PyObject* const* args) {
                    static_cast<uint16_t*>(out.data_ptr()), want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr,
                    bytes ? ws.data_ptr() : nullptr, bytes, c10::cuda::getCurrentCUDAStream(p.index).stream()),
           "fkv_paged_attend");
+    written(out0);
     if (!want_lse) return THPVariable_Wrap(out);
     PyObject* r = PyTuple_New(2);
     PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));

@@ -386,7 +386,7 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
     const int passes = (std::max(c->Hk, n->Hq) + rows - 1) / rows;
     // few tokens: their rows are spread over more blocks
     a.per_block = std::min(tokens_per_block(n->T, 2 * c->Hk + n->Hq), rows);
-    const dim3 grid((n->T + a.per_block - 1) / a.per_block, std::min(passes, std::max(1, 592 / n->T)));
+    const dim3 grid((n->T - 1) / a.per_block + 1, std::min(passes, std::max(1, 592 / n->T)));
     const size_t smem = (size_t)a.per_block * a.half * 2 * sizeof(float);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool il = n->interleaved != 0;

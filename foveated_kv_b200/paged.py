@@ -81,7 +81,7 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     """Attention of one new token per sequence over its pages.
 
     q (B, Hq, D) or (B, Hq, 1, D), Hq a multiple of Hk; ``scale`` 1/sqrt(D) by
-    default; ``window`` > 0 attends the last ``window`` tokens only.  Returns
+    default; the pages' own scales are not negative; ``window`` > 0 attends the last ``window`` tokens only.  Returns
     out, of q's shape, and with return_lse the natural log-sum-exp of the
     scaled scores, (B, Hq) float32.  A sequence without tokens gives zeros and
     -inf.  A score of +inf gives NaN and +inf; an infinite value gives a
@@ -190,7 +190,8 @@ class PagedKVCache:
             raise ValueError(f"slot {slot} of {self.max_seqs}")
 
     def release(self, slot: int) -> None:
-        """Empty a slot; its pages may be given to other sequences."""
+        """Empty a slot, between steps; its pages may be given to other
+        sequences."""
         self._check_slot(slot)
         self._free.extend(reversed(self._pages[slot]))
         self._pages[slot] = []

@@ -703,3 +703,45 @@ assert torch.equal(d[1][0, :, 299], k[0])
 """
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=root)
+
+
+def test_written_tensors_beside_autograd():
+    """A graph that saved a tensor written here says so in its backward pass;
+    outputs that overlap the pages, or require a gradient, are refused."""
+    p = R.Pages(51, [20, 30], 2, 64, 16, F16, False)
+    e = R.Pages(51, [20, 30], 2, 64, 16, F16, True)
+    f, pos = fkv.rotary_frequencies(64)[0], torch.arange(2, device="cuda")
+    q, k = _rand(2, 4, 64, dtype=F16), _rand(2, 2, 64, dtype=F16, seed=1)
+    cases = [
+        (q, lambda: fkv.apply_rotary(q, None, pos, f, out=q)),
+        (k, lambda: fkv.apply_rotary(q, k, pos, f, out=(q, k))),
+        (q, lambda: fkv.paged_attend(q.clone(), out=q, **p.kw)),
+        (q, lambda: fkv.paged_append(k, k, q=q, q_out=q, inv_freq=f, **p.kw)),
+        (p.v_pages, lambda: fkv.paged_append(k, k, **p.kw)),
+        (e.k_scale, lambda: fkv.paged_append(k, k, **e.kw)),
+    ]
+    for saved, write in cases:
+        w = torch.ones((), dtype=saved.dtype, device="cuda", requires_grad=True)
+        y = (w * saved).sum()
+        write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        i = _rand(2, 4, 64, dtype=F16)
+    fkv.apply_rotary(i, None, pos, f, out=i)                     # no version to count
+    grad = torch.zeros(2, 4, 64, dtype=F16, device="cuda", requires_grad=True)
+    rows = p.k_pages.view(-1)[:2 * 4 * 64].view(2, 4, 64)
+    for write in (lambda: fkv.apply_rotary(q, None, pos, f, out=grad), lambda: fkv.paged_attend(q, out=grad, **p.kw),
+                  lambda: fkv.paged_attend(q, out=rows, **p.kw),
+                  lambda: fkv.paged_attend(q, **dict(p.kw, k_pages=p.k_pages.clone().requires_grad_())),
+                  lambda: fkv.paged_append(k, k, q=q, q_out=rows, inv_freq=f, **p.kw)):
+        with pytest.raises(ValueError):
+            write()
+    with torch.no_grad():
+        fkv.paged_attend(q, out=grad, **p.kw)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_attend_scale_of_any_sign(scale, fp8):
+    _attend(R.Pages(52, [1, 40, 900], 2, 128, 16, BF16, fp8), 8, scale=scale)
