@@ -3,8 +3,9 @@
 // decode wants every sequence of a batch to have one length).
 //
 //   out[h] = sum_n p_n v_n / sum_n p_n,  p_n = exp(scale q[h].k_n - m),
-//   n over the last `window` (or all) tokens of the sequence; a sequence
-//   without tokens gives zeros and a log-sum-exp of -inf.
+//   n over the last `window` (or all) tokens of the sequence that have a page;
+//   a sequence without such tokens gives zeros and a log-sum-exp of -inf, one
+//   whose scores are all -inf NaN (0 / 0) and -inf.
 //
 // Work split.  A stream is one (sequence, kv head, group of up to 16 query
 // heads); its tokens are cut into units of 64 or 128.  The units of all
@@ -69,7 +70,7 @@ struct AttendArgs {
     uint16_t* out;
     float* lse;
     float* rec_o;      // (2 per CTA, HP heads, D)
-    float4* rec_s;     // (2 per CTA, HP heads): m, M, l
+    float4* rec_s;     // (2 per CTA, HP heads): m, M, l, 1 if it attended any token
     int4* desc;        // first output row, heads, pieces (0: nothing to join), first record
     int Hq, G, HT, pshift, window, per_stream, wave, waves;
     float sl2;         // scale * log2(e)
@@ -292,6 +293,7 @@ template <int D, int HP>
 struct Join {
     float o[kWarps][HP][D + 2];
     float m[kWarps][HP], M[kWarps][HP], l[kWarps][HP];
+    int any[kWarps];     // a token was there
 };
 
 template <int D, int HP, int KIND>
@@ -500,13 +502,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
         // DIRECT: the lane's pieces of the tile at t0, rows g of K and 2t, 2t + 1 of
         // V of every 8-token group; rows outside [lo, t_end) become zeros
         uint4 kr[TG][2][KC], vr[TG][4][VC];
-        uint32_t live = 0;     // rows g to attend, a bit for each 8-token group
+        // rows g to attend, a bit for each 8-token group; the sign stays once any tile
+        // had one (a flag of its own spilled registers)
+        uint32_t live = 0;
         auto is_full = [&](int t0, uint32_t lines) {
             return __all_sync(0xffffffffu, lines != ~0u || lane >= 2 * TG) && t0 >= lo && t0 + GG::ROWS <= t_end;
         };
         auto load_k = [&](int t0, uint32_t lines) {
             const bool full = is_full(t0, lines);
-            live = ~0u;
+            live = full ? ~0u : live & 0x80000000u;
 #pragma unroll
             for (int k = 0; k < 2 * TG; ++k) {
                 const uint32_t line = __shfl_sync(0xffffffffu, lines, k);
@@ -518,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
                 } else {
                     const int tok = t0 + 8 * k + g;
                     const bool ok = line != ~0u && tok >= lo && tok < t_end;
-                    if (!ok) live &= ~(1u << k);
+                    if (ok) live |= 0x80000000u | 1u << k;
 #pragma unroll
                     for (int cc = 0; cc < KC; ++cc) {
                         kr[k >> 1][k & 1][cc] = make_uint4(0, 0, 0, 0);
@@ -554,6 +558,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
         int t0 = t_begin + warp * 16 * TG;
         uint32_t buf = 0;      // offset of the tile's buffer
         uint32_t lines = group_of(t0);
+        bool seen = false;
         if constexpr (DIRECT) {
             load_k(t0, lines);
             load_v(t0, lines);
@@ -667,7 +672,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
             float av[TG][2];      // log2 of the values' scales
             float top[NT][2], topw[NT][2];
             uint32_t have = live;
-            if constexpr (!DIRECT) have = lds4(cur + GG::OFF_L);
+            if constexpr (!DIRECT) {
+                have = lds4(cur + GG::OFF_L);
+                seen |= have != 0;
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = topw[nt][0] = topw[nt][1] = -INFINITY;
 #pragma unroll
@@ -828,7 +836,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
 
         // ---- join the warps -----------------------------------------------------------------------
         copies_wait<0>();
+        const bool any = __any_sync(0xffffffffu, DIRECT ? live >> 31 : seen);
         __syncthreads();                 // the buffers' memory changes hands
+        if (lane == 0) sm.any[warp] = any;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -851,6 +861,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
             }
         __syncthreads();
         const bool whole = chunk == 0 && chunk_end == nu;
+        int attended = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) attended |= sm.any[w];
         const int slot = 2 * blockIdx.x + (u == u0 ? 0 : 1);
         for (int i = tid; i < nh * (D / 2); i += kThreads) {
             const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
@@ -868,8 +881,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
                 y1 += sm.o[w][h][d + 1] * f;
             }
             if (whole) {
-                // all scores -inf: l = 0 and the quotient is NaN, as the formula's
-                const float f = (KIND == FP8 && MM != -INFINITY && mm != -INFINITY ? ex2(MM - mm) : 1.f) / ll;
+                // all scores -inf: l = 0 and the quotient is NaN, as the formula's;
+                // no token at all: zeros
+                const float f = (KIND == FP8 && MM != -INFINITY && mm != -INFINITY ? ex2(MM - mm) : 1.f) /
+                                (attended ? ll : 1.f);
                 y0 *= f;
                 y1 *= f;
                 const int64_t at = (row0 + h) * D + d;
@@ -878,7 +893,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
             } else {
                 const int64_t at = (int64_t)slot * HP + h;
                 *reinterpret_cast<float2*>(a.rec_o + at * D + d) = make_float2(y0, y1);
-                if (d == 0) a.rec_s[at] = make_float4(mm, MM, ll, 0.f);
+                if (d == 0) a.rec_s[at] = make_float4(mm, MM, ll, attended ? 1.f : 0.f);
             }
         }
         if (a.desc && chunk == 0 && tid == 0) {
@@ -908,7 +923,7 @@ template <int D>
 __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__ AttendArgs a, int HP, bool fp8) {
     constexpr int VE = D / 32, BATCH = 8;
     __shared__ float so[kJoinMost / 32][D];
-    __shared__ float ss[kJoinMost / 32][3];
+    __shared__ float ss[kJoinMost / 32][4];
     await_predecessor();
     const int4 ds = a.desc[blockIdx.x];
     const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -924,7 +939,7 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
     struct alignas(4 * (VE < 4 ? VE : 4)) Row {
         float v[VE];
     };
-    float m = -INFINITY, M = -INFINITY, l = 0.f, o[VE];
+    float m = -INFINITY, M = -INFINITY, l = 0.f, any = 0.f, o[VE];
 #pragma unroll
     for (int e = 0; e < VE; ++e) o[e] = 0.f;
     for (int i0 = 0; i0 < mine; i0 += 32) {
@@ -948,6 +963,7 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
         Mn = fmaxf(M, Mn);
         const float fl = m == -INFINITY ? 1.f : ex2(m - mn), fo = M == -INFINITY ? 1.f : ex2(M - Mn);
         l = l * fl + s.z * (s.x == -INFINITY ? 1.f : ex2(s.x - mn));
+        any = fmaxf(any, s.w);
         const float w = s.y == -INFINITY ? 1.f : ex2(s.y - Mn);
 #pragma unroll
         for (int e = 0; e < VE; ++e) o[e] *= fo;
@@ -967,6 +983,7 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
     }
 #pragma unroll
     for (int k = 16; k > 0; k >>= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+    any = __any_sync(0xffffffffu, any != 0.f) ? 1.f : 0.f;
     if (!alone) {
 #pragma unroll
         for (int e = 0; e < VE; ++e) so[warp][lane * VE + e] = o[e];
@@ -974,6 +991,7 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
             ss[warp][0] = m;
             ss[warp][1] = M;
             ss[warp][2] = l;
+            ss[warp][3] = any;
         }
         __syncthreads();
         if (warp > 0) return;
@@ -981,6 +999,7 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
         for (int w = 0; w < warps; ++w) {
             mm = fmaxf(mm, ss[w][0]);
             MM = fmaxf(MM, ss[w][1]);
+            any = fmaxf(any, ss[w][3]);
         }
 #pragma unroll
         for (int e = 0; e < VE; ++e) o[e] = 0.f;
@@ -994,7 +1013,7 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
         M = MM;
         l = ll;
     }
-    const float f = (fp8 && M != -INFINITY && m != -INFINITY ? ex2(M - m) : 1.f) / l;
+    const float f = (fp8 && M != -INFINITY && m != -INFINITY ? ex2(M - m) : 1.f) / (any != 0.f ? l : 1.f);
     uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (int64_t)(ds.x + h) * D) + lane * (VE / 2);
 #pragma unroll
     for (int e = 0; e < VE; e += 2)

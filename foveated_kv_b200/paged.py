@@ -83,8 +83,8 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     q (B, Hq, D) or (B, Hq, 1, D), Hq a multiple of Hk; ``scale`` 1/sqrt(D) by
     default; the pages' own scales are not negative; ``window`` > 0 attends the last ``window`` tokens only.  Returns
     out, of q's shape, and with return_lse the natural log-sum-exp of the
-    scaled scores, (B, Hq) float32.  A sequence without tokens gives zeros and
-    -inf.  A score of +inf gives NaN and +inf; an infinite value gives a
+    scaled scores, (B, Hq) float32.  A sequence without tokens, or with none that
+    has a page, gives zeros and -inf.  A score of +inf gives NaN and +inf; an infinite value gives a
     non-finite output.  Lengths are read on the device, so the call can be
     captured once and replayed as sequences grow within the table; neither they
     nor the table may change while it runs.  The work split follows the table's

@@ -395,10 +395,10 @@ int fkv_paged_read(const FkvPagedCache* c, int32_t max_len, uint16_t* k, uint16_
 
 /* Attention of one token per sequence over its last `window` tokens (0: all):
  * q, out (B, Hq, D) 16-bit, 16-byte aligned; lse (B, Hq) f32 natural
- * log-sum-exp of the scaled scores, or NULL.  A sequence without tokens gives
- * zeros and -inf.  table and lens must not change while the launch runs, and
- * out must not overlap q.  The workspace needs no initialisation; calls that
- * share one must not overlap on the GPU. */
+ * log-sum-exp of the scaled scores, or NULL.  A sequence without tokens, or
+ * with none that has a page, gives zeros and -inf.  table and lens must not
+ * change while the launch runs, and out must not overlap q.  The workspace
+ * needs no initialisation; calls that share one must not overlap on the GPU. */
 size_t fkv_paged_attend_workspace_bytes(const FkvPagedCache* c, int32_t Hq);
 int fkv_paged_attend(const FkvPagedCache* c, int32_t Hq, float scale, int32_t window,
                      const uint16_t* q, uint16_t* out, float* lse, void* workspace,

@@ -1,0 +1,78 @@
+"""Edges of the paged cache's and rotary calls on the GPU: tokens that are left
+out, lengths that are none, weights far below the largest, calls that are
+refused."""
+
+import math
+
+import pytest
+import torch
+
+import foveated_kv_b200 as fkv
+from foveated_kv_b200 import FkvNativeError, PagedKVCache
+from tests import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F8 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
+INF = float("inf")
+
+
+def _rand(*shape, dtype, seed=0):
+    return torch.randn(*shape, generator=torch.Generator("cuda").manual_seed(seed), device="cuda").to(dtype)
+
+
+def _status():
+    return torch.zeros(1, dtype=torch.int32, device="cuda")
+
+
+# ---- attention: tokens left out -----------------------------------------------------------------
+
+@pytest.mark.parametrize("D,G", [(64, 4), (64, 16), (128, 8), (256, 2)])
+@pytest.mark.parametrize("dtype,fp8", [(F16, False), (BF16, False), (F16, True), (BF16, True)])
+@pytest.mark.parametrize("n", [40, 30000])                       # one CTA's work, many CTAs'
+def test_tokens_all_left_out(n, dtype, fp8, D, G):
+    """No table entry that is a page: as a sequence without tokens."""
+    p = R.Pages(1, [n, 33, 5], 2, D, 16, dtype, fp8, width_extra=0)
+    q = _rand(3, 2 * G, D, dtype=dtype)
+    want, wlse = fkv.paged_attend(q, return_lse=True, **p.kw)
+    t, st = p.table.clone(), _status()
+    t[0] = -1
+    out, lse = fkv.paged_attend(q, return_lse=True, status=st, **dict(p.kw, table=t))
+    assert st.item() == 1 and (out[0] == 0).all() and (lse[0] == -INF).all()
+    assert torch.equal(out[1:], want[1:]) and torch.equal(lse[1:], wlse[1:])
+    t = p.table.clone()                                          # a window wholly on bad pages
+    t[0, (n - 20) // 16:] = p.k_pages.shape[0]
+    out, lse = fkv.paged_attend(q, return_lse=True, window=20, **dict(p.kw, table=t))
+    assert (out[0] == 0).all() and (lse[0] == -INF).all() and torch.isfinite(out[1:]).all()
+    t = p.table.clone()                                          # the first half left out
+    cut = n // 32 * 16
+    t[0, :cut // 16] = -1
+    out, lse = fkv.paged_attend(q, return_lse=True, **dict(p.kw, table=t))
+    ref, rlse, mag, dot = R.attend(q, [x[:, cut if b == 0 else 0:] for b, x in enumerate(p.sequences("k"))],
+                                   [x[:, cut if b == 0 else 0:] for b, x in enumerate(p.sequences("v"))], [n - cut, 33, 5])
+    slack = R.attend_slack(dtype, fp8, [n], dot, mag, 6.0)
+    tol = R.HALF_STEP[dtype] * (ref.abs() + slack) + slack + R.SUBNORMAL[dtype]
+    assert ((out.double() - ref).abs() <= tol).all()
+    assert (lse.double() - rlse).abs().max() <= 2.0 ** -18 * float(dot.max()) + (n / 16 + 64) * 2.0 ** -22
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_tokens_of_an_empty_pool(fp8):
+    p = R.Pages(2, [0, 0], 2, 64, 16, F16, fp8, spare=0)
+    kw = dict(p.kw, lens=torch.tensor([20, 3], dtype=torch.int32, device="cuda"), table=p.table.abs())
+    out, lse = fkv.paged_attend(_rand(2, 4, 64, dtype=F16), return_lse=True, **kw)
+    assert (out == 0).all() and (lse == -INF).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n", [40, 30000])
+def test_scores_all_minus_infinity(n, dtype):
+    """Tokens that are there with scores of -inf are not left out: 0 / 0, with
+    a log-sum-exp of -inf, beside pages that are missing as without them."""
+    p = R.Pages(3, [n], 1, 64, 16, dtype, False, width_extra=0)
+    p.k_pages[p.table[0].long()] = -INF
+    q = _rand(1, 4, 64, dtype=dtype).abs() + 0.1
+    t = p.table.clone()
+    t[0, 1:-1] = -1
+    for table in (p.table, t):
+        out, lse = fkv.paged_attend(q, return_lse=True, **dict(p.kw, table=table))
+        assert torch.isnan(out).all() and (lse == -INF).all()
