@@ -346,7 +346,7 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
     FKV_REQUIRE(n->Hq == 0 || n->rot != 0, FKV_ERR_INVALID, "fkv_paged_append: queries without a rotation");
     FKV_REQUIRE(c->Hk <= 4096 && n->Hq <= 8192, FKV_ERR_UNSUPPORTED, "fkv_paged_append: %d / %d heads are too many",
                 c->Hk, n->Hq);
-    if (n->T == 0 || c->B == 0) return FKV_OK;
+    if (n->T == 0) return FKV_OK;
     FKV_REQUIRE(n->k && n->v && (n->Hq == 0 || (n->q && n->q_out)) && (n->rot == 0 || n->inv_freq),
                 FKV_ERR_INVALID, "fkv_paged_append: NULL pointer");
     AppendArgs a;
@@ -370,6 +370,18 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
             wide = wide && st[i][j] % 8 == 0;
         }
     }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (c->B == 0) {             // packed rows of no sequence: padding, whose queries are zeros
+        const int64_t tok = a.qos[1], head = a.qos[2];
+        const size_t row = c->D * sizeof(uint16_t);
+        const bool packed = head == c->D;        // a token's heads in a row
+        for (int h = 0; h < (packed ? std::min(n->Hq, 1) : n->Hq); ++h) {
+            const size_t width = packed ? n->Hq * row : row;
+            const size_t pitch = n->T > 1 ? (size_t)tok * sizeof(uint16_t) : width;
+            FKV_CUDA_CHECK(cudaMemset2DAsync(n->q_out + h * head, pitch, 0, width, n->T, s));
+        }
+        return FKV_OK;
+    }
     a.k = n->k;
     a.v = n->v;
     a.q = n->q;
@@ -388,7 +400,6 @@ extern "C" int fkv_paged_append(const FkvPagedCache* c, const FkvPagedNew* n, vo
     a.per_block = std::min(tokens_per_block(n->T, 2 * c->Hk + n->Hq), rows);
     const dim3 grid((n->T - 1) / a.per_block + 1, std::min(passes, std::max(1, 592 / n->T)));
     const size_t smem = (size_t)a.per_block * a.half * 2 * sizeof(float);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool il = n->interleaved != 0;
     FKV_CUDA_CHECK(c->D == 64    ? launch_append<64>(a, grid, smem, il, wide, s)
                    : c->D == 128 ? launch_append<128>(a, grid, smem, il, wide, s)

@@ -76,3 +76,26 @@ def test_scores_all_minus_infinity(n, dtype):
     for table in (p.table, t):
         out, lse = fkv.paged_attend(q, return_lse=True, **dict(p.kw, table=table))
         assert torch.isnan(out).all() and (lse == -INF).all()
+
+
+# ---- writing ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,fp8", [(F16, False), (BF16, True)])
+def test_append_of_padding_alone(dtype, fp8):
+    """No sequences at all, rows of padding: their queries are zeros."""
+    p = R.Pages(6, [20], 2, 64, 16, dtype, fp8)
+    before = [x.view(torch.uint8).clone() for x in (p.k_pages, p.v_pages)]
+    kw = dict(p.kw, table=p.table[:0], lens=p.lens[:0])
+    cu = torch.zeros(1, dtype=torch.int32, device="cuda")
+    k, q = _rand(700, 2, 64, dtype=dtype), _rand(700, 6, 64, dtype=dtype)
+    f, st = fkv.rotary_frequencies(64)[0], _status()
+    new = lambda *shape: torch.full(shape, 7.0, dtype=dtype, device="cuda")
+    wide = new(700, 9, 64)
+    for got in (new(700, 6, 64), wide[:, 1:7], new(6, 700, 64).transpose(0, 1)):
+        fkv.paged_append(k, k, cu_new=cu, q=q, q_out=got, inv_freq=f, status=st, **kw)
+        assert (got == 0).all() and st.item() == 0
+    assert (wide[:, 0] == 7).all() and (wide[:, 7:] == 7).all()
+    assert (fkv.paged_append(k[:1], k[:1], cu_new=cu, q=q[:1], inv_freq=f, **kw) == 0).all()
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, (p.k_pages, p.v_pages)))
+    fkv.paged_append(k, k, cu_new=cu, **kw)
+    fkv.paged_append(k[:0], k[:0], **kw)
