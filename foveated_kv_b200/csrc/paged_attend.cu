@@ -39,7 +39,7 @@
 //
 // 8-bit rows: codes become f16 exactly.  A key's scale multiplies its score.
 // A value's scale joins the exponent: w_n = exp2(x_n + log2 s_n - M) with a
-// running maximum M of its own, so w never leaves the range of f16 however
+// running maximum M of its own, so w never passes the range of f16 however
 // large or small the scales are, and the result is (sum w_n c_n) 2^(M-m) / l.
 #include <algorithm>
 #include <atomic>
@@ -60,9 +60,19 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr uint32_t kFull = 0xFFFFFFFFu;
-constexpr float kLazy = 8.f;          // log2 units a running maximum may lag behind
-
 enum { F16 = 0, BF16 = 1, FP8 = 2 };  // what the pages hold
+
+// A running maximum may lag kLazy log2 units behind the scores.  Weights that
+// enter the tensor core as f16 (beside f16 and 8-bit pages) are held times
+// 2^kLift, up to 2^15 with the lag, and so is their sum: f16 holds them to half
+// of 2^-24, which is 2^-36 of the largest weight.  Unlifted, 2^-25 of it, many
+// small weights together were lost (500 tokens at 2^-25 of one whose value is
+// zero: a quarter of the output); it costs up to 1.3 % (8 x 64K fp8, 16 heads a
+// group: 72.4 -> 73.5 us).  bf16 has the range of f32, and its values need the room.
+template <int KIND>
+constexpr float kLift = KIND == BF16 ? 0.f : 11.f;
+template <int KIND>
+constexpr float kLazy = KIND == BF16 ? 8.f : 4.f;
 
 struct AttendArgs {
     FkvPagedCache c;
@@ -89,9 +99,9 @@ __device__ __forceinline__ float lg2(float x) {
 // 2^(a - b) where b is a maximum over a: 0 for an empty side
 __device__ __forceinline__ float ratio2(float a, float b) { return a == -INFINITY ? 0.f : ex2(a - b); }
 
-// natural log of l 2^m; +inf where a score is (the weights are NaN then)
-__device__ __forceinline__ float log_sum(float m, float l) {
-    return m == INFINITY ? m : (m + log2f(l)) * 0.6931471805599453f;
+// natural log of l 2^(m - lift); +inf where a score is (the weights are NaN then)
+__device__ __forceinline__ float log_sum(float m, float l, float lift) {
+    return m == INFINITY ? m : (m + (log2f(l) - lift)) * 0.6931471805599453f;
 }
 
 // (not .nc: an early launch's data may be written while the grid already waits)
@@ -709,8 +719,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
-                    up |= top[nt][i] > m[nt][i] + kLazy;
-                    if (KIND == FP8) up |= topw[nt][i] > M[nt][i] + kLazy;
+                    up |= top[nt][i] > m[nt][i] + kLazy<KIND>;
+                    if (KIND == FP8) up |= topw[nt][i] > M[nt][i] + kLazy<KIND>;
                 }
             if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -748,13 +758,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
             // 64 x 32K goes from 507 to 516 us, 592 to 617 under the power cap.
             // The first part is cut off below the weight, so that both are
             // positive and an infinite value gives an infinity, not the NaN of
-            // inf - inf (f16: for weights from 2^-14 of the largest; under that
+            // inf - inf (f16: for weights from 2^-25 of the largest; under that
             // the second part may be zero)
             uint32_t pf[TG][NT][2], pl[TG][NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-                const float M0 = M[nt][0] == -INFINITY ? 0.f : M[nt][0], M1 = M[nt][1] == -INFINITY ? 0.f : M[nt][1];
+                auto base = [](float x) { return (x == -INFINITY ? 0.f : x) - kLift<KIND>; };
+                const float m0 = base(m[nt][0]), m1 = base(m[nt][1]), M0 = base(M[nt][0]), M1 = base(M[nt][1]);
 #pragma unroll
                 for (int tg = 0; tg < TG; ++tg)
 #pragma unroll
@@ -889,7 +899,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<D, HP>) attend_kernel(const _
                 y1 *= f;
                 const int64_t at = (row0 + h) * D + d;
                 *reinterpret_cast<uint32_t*>(a.out + at) = bf ? pack2<true>(y0, y1) : pack2<false>(y0, y1);
-                if (a.lse && d == 0) a.lse[row0 + h] = log_sum(mm, ll);
+                if (a.lse && d == 0) a.lse[row0 + h] = log_sum(mm, ll, kLift<KIND>);
             } else {
                 const int64_t at = (int64_t)slot * HP + h;
                 *reinterpret_cast<float2*>(a.rec_o + at * D + d) = make_float2(y0, y1);
@@ -1018,7 +1028,7 @@ __global__ void __launch_bounds__(kJoinMost) join_kernel(const __grid_constant__
 #pragma unroll
     for (int e = 0; e < VE; e += 2)
         dst[e / 2] = a.c.bf16 ? pack2<true>(o[e] * f, o[e + 1] * f) : pack2<false>(o[e] * f, o[e + 1] * f);
-    if (a.lse && lane == 0) a.lse[ds.x + h] = log_sum(m, l);
+    if (a.lse && lane == 0) a.lse[ds.x + h] = log_sum(m, l, fp8 || !a.c.bf16 ? kLift<F16> : kLift<BF16>);
 }
 
 // Streams of up to so many units stay whole, a CTA each: no records, no second

@@ -78,6 +78,38 @@ def test_scores_all_minus_infinity(n, dtype):
         assert torch.isnan(out).all() and (lse == -INF).all()
 
 
+# ---- attention: weights far below the largest ---------------------------------------------------
+
+@pytest.mark.parametrize("bits", [20, 25, 28])
+@pytest.mark.parametrize("dtype,fp8", [(F16, False), (BF16, False), (F16, True), (BF16, True)])
+@pytest.mark.parametrize("n", [500, 30000])
+def test_many_small_weights(n, dtype, fp8, bits):
+    """One token with a value of zero takes most of the weight, the others
+    2^-bits of it each: the output is the others' sum."""
+    p = R.Pages(4, [n], 1, 64, 16, dtype, fp8)
+    for x in (p.k_pages, p.v_pages):
+        x.view(torch.uint8).zero_()
+    ids = p.table[0, :-(-n // 16)].long()
+    first = ids[0]
+    p.k_pages[first, 0, 0, 0] = 1.0
+    v = torch.rand(len(ids), 1, 16, 64, generator=torch.Generator("cuda").manual_seed(5), device="cuda") + 0.5
+    v[0, :, 0] = 0.0
+    p.v_pages[ids] = (v * (256 if fp8 else 16384)).to(p.v_pages.dtype)
+    if fp8:
+        p.k_scale.fill_(1.0)
+        p.v_scale.fill_(64.0)
+    q = torch.zeros(1, 4, 64, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    scale = bits * math.log(2.0)
+    out = fkv.paged_attend(q, scale=scale, **p.kw).double()
+    ref, _, mag, dot = R.attend(q, p.sequences("k"), p.sequences("v"), [n], 0, scale)
+    slack = R.attend_slack(dtype, fp8, [n], dot, mag, 0.0)
+    if fp8 or dtype is F16:
+        # a part of a weight below f16's normal numbers is off by up to 2^-25 / 2^11, where the largest weight is at least 1
+        slack = slack + n * 2.0 ** -36 * 24576.0
+    assert ((out - ref).abs() <= R.HALF_STEP[dtype] * (ref.abs() + slack) + slack + R.SUBNORMAL[dtype]).all()
+
+
 # ---- writing ------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,fp8", [(F16, False), (BF16, True)])
