@@ -11,6 +11,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -89,12 +90,17 @@ int32_t size32(int64_t v, const char* who) {
 bool is16(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 int index_of(const Tensor& t) { return t.is_cuda() ? (int)t.get_device() : -1; }
 
-// these operators serve; they carry no gradient
+// these operators serve; they carry no gradient, neither back nor forward (the
+// tangent of a dual tensor)
 void refuse_grad(const char* who, std::initializer_list<const Tensor*> ts) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor* t : ts)
-        require(t == nullptr || !t->requires_grad(), who,
+    const bool back = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const Tensor* t : ts) {
+        if (t == nullptr) continue;
+        require(!back || !t->requires_grad(), who,
                 "inputs that require a gradient are not supported (call it under torch.no_grad())");
+        require(!forward || !t->_fw_grad(0).defined(), who,
+                "inputs with a tangent (forward gradient) are not supported");
+    }
 }
 
 // 16-bit rows that the kernels can address: contiguous heads, 8-byte aligned,
@@ -182,7 +188,7 @@ PyObject* rotary(PyObject* const* args) {
     const auto dt = q.scalar_type();
     require(index >= 0, who, "q must be a CUDA tensor");
     require(is16(dt), who, "q is ", dt, ", expected float16 or bfloat16");
-    refuse_grad(who, {&q, k, q_out, k_out});
+    refuse_grad(who, {&q, k, &f, q_out, k_out});
     const int64_t nd = q.dim();
     require(nd == 3 || nd == 4, who, "q must be (B, H, S, D) or (T, H, D), got ", q.sizes());
     FkvRotaryShape sh = {};
@@ -312,7 +318,7 @@ PyObject* append(PyObject* const* args) {
     const Tensor &k = tensor(args[7], who, "k"), &v = tensor(args[8], who, "v");
     const Tensor *cu = maybe(args[9], who, "cu_new"), *q = maybe(args[10], who, "q");
     const Tensor *f = maybe(args[11], who, "inv_freq"), *q_out = maybe(args[14], who, "q_out");
-    refuse_grad(who, {&k, &v, q, q_out});
+    refuse_grad(who, {&k, &v, q, f, q_out});
     const auto dt = k.scalar_type();
     const Pages p = pages(who, args, dt);
     const int64_t nd = k.dim();

@@ -131,3 +131,30 @@ def test_append_of_padding_alone(dtype, fp8):
     assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, (p.k_pages, p.v_pages)))
     fkv.paged_append(k, k, cu_new=cu, **kw)
     fkv.paged_append(k[:0], k[:0], **kw)
+
+
+# ---- gradients ----------------------------------------------------------------------------------
+
+def test_frequencies_and_tangents_are_refused():
+    p = R.Pages(7, [20, 30], 2, 64, 16, F16, False)
+    q, k = _rand(2, 4, 64, dtype=F16), _rand(2, 2, 64, dtype=F16)
+    pos, f = torch.arange(2, device="cuda"), fkv.rotary_frequencies(64)[0]
+    g = f.clone().requires_grad_()
+    rotary = lambda **kw: fkv.apply_rotary(**dict(dict(q=q, k=k, positions=pos, inv_freq=f), **kw))
+    append = lambda **kw: fkv.paged_append(**dict(dict(k=k, v=k.clone(), q=q, inv_freq=f, **p.kw), **kw))
+    attend = lambda **kw: fkv.paged_attend(**dict(dict(q=q, **p.kw), **kw))
+    for call in (lambda: rotary(inv_freq=g), lambda: append(inv_freq=g)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    ad = torch.autograd.forward_ad
+    with ad.dual_level():
+        dual = lambda x: ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: rotary(q=dual(q)), lambda: rotary(k=dual(k)), lambda: rotary(inv_freq=dual(f)),
+                     lambda: rotary(out=(dual(q.clone()), k.clone())), lambda: append(k=dual(k)), lambda: append(v=dual(k)),
+                     lambda: append(q=dual(q)), lambda: append(inv_freq=dual(f)), lambda: attend(q=dual(q)),
+                     lambda: attend(k_pages=dual(p.k_pages)), lambda: attend(out=dual(torch.empty_like(q)))):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+        rotary(), append(), attend()
