@@ -286,11 +286,10 @@ constexpr int kPerSm = D == 256 || HP == 16 ? 2 : 3;
 __device__ __forceinline__ void seq_range(const AttendArgs& a, int b, int& lo, int& len) {
     const int reach = a.c.width << a.pshift;
     len = a.c.lens[b];
-    if (len > reach) {
+    if ((unsigned)len > (unsigned)reach) {       // or below zero
         paged_report(a.c.status, FKV_PAGED_BAD_POSITION);
-        len = reach;
+        len = len < 0 ? 0 : reach;
     }
-    len = max(len, 0);
     lo = a.window > 0 ? max(0, len - a.window) : 0;
 }
 template <int UNIT>

@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
     const int b = (int)(bh / a.c.Hk), h = (int)(bh - (int64_t)b * a.c.Hk);
     const int64_t reach = (int64_t)a.c.width << a.pshift;
     const int len = a.c.lens[b];
-    if (len > reach && threadIdx.x == 0 && chunk == 0 && h == 0)
+    if ((len < 0 || len > reach) && threadIdx.x == 0 && chunk == 0 && h == 0)
         paged_report(a.c.status, FKV_PAGED_BAD_POSITION);
     const int n = (int)min((int64_t)min(len, a.max_len), reach);
     const int32_t* tab = a.c.table + (int64_t)b * a.c.table_stride;

@@ -18,7 +18,7 @@ Tensors shared by the three functions, P pages of ``page`` tokens:
   lens              (B,) int32: tokens of each sequence, new ones included
   status            optional int32 word of sticky error bits: 1 = a table entry
                     that is no page (its tokens are left out), 2 = a length or
-                    position outside the table
+                    position below zero or outside the table
 """
 
 from __future__ import annotations

@@ -361,7 +361,7 @@ typedef struct FkvPagedCache {
 } FkvPagedCache;
 
 #define FKV_PAGED_BAD_PAGE 1     /* a table entry that is no page: its tokens are left out */
-#define FKV_PAGED_BAD_POSITION 2 /* a length or position outside the table's reach */
+#define FKV_PAGED_BAD_POSITION 2 /* a length or position below zero or outside the table's reach */
 
 /* New tokens, (token, head) rows with any strides (multiples of 4 elements,
  * pointers 8-byte aligned).  cu_new == NULL: n_uniform tokens for each of the

@@ -110,6 +110,26 @@ def test_many_small_weights(n, dtype, fp8, bits):
     assert ((out - ref).abs() <= R.HALF_STEP[dtype] * (ref.abs() + slack) + slack + R.SUBNORMAL[dtype]).all()
 
 
+# ---- lengths below zero -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", [64, 30000])
+def test_negative_lengths_are_reported(n, fp8):
+    p = R.Pages(5, [5, n, 9], 2, 64, 16, F16, fp8)
+    q, st = _rand(3, 4, 64, dtype=F16), _status()
+    want = fkv.paged_attend(q, status=st, **p.kw)
+    assert st.item() == 0
+    for bad in (-1, -2 ** 31):
+        kw = dict(p.kw, lens=torch.tensor([bad, n, 9], dtype=torch.int32, device="cuda"))
+        out, lse = fkv.paged_attend(q, status=st, return_lse=True, **kw)
+        assert st.item() == 2 and (out[0] == 0).all() and (lse[0] == -INF).all()
+        assert (out[1:].double() - want[1:].double()).abs().max() < 2.0 ** -8    # the work is split otherwise
+        st.zero_()
+        k, v = fkv.paged_read(max_len=9, dtype=F16, status=st, **kw)
+        assert st.item() == 2 and (k[0] == 0).all() and (v[0] == 0).all()
+        st.zero_()
+
+
 # ---- writing ------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype,fp8", [(F16, False), (BF16, True)])
