@@ -207,6 +207,9 @@ class PagedKVCache:
             raise ValueError("append: call extend first")
         if k.shape[0] != self._new_rows if not self._packed else k.shape[0] < self._new_rows:
             raise ValueError(f"append: {k.shape[0]} rows of k, the step has {self._new_rows}")
+        if k.dim() == 4 and (self._packed or k.shape[2] != 1):
+            raise ValueError(f"append: k {tuple(k.shape)}, expected (rows, H_kv, D)" +
+                             ("" if self._packed else " or (slots, H_kv, 1, D)"))
         turn = {} if self.inv_freq is None else dict(inv_freq=self.inv_freq, interleaved=self.interleaved,
                                                      amplitude=self.amplitude, q=q)
         lens, cu = (self.lens, self._cu) if self._packed else (self._step_lens, None)

@@ -153,6 +153,29 @@ def test_append_of_padding_alone(dtype, fp8):
     fkv.paged_append(k[:0], k[:0], **kw)
 
 
+def test_cache_takes_one_row_per_slot():
+    """A step of single tokens given as (slots, heads, n, D) with n other than 1
+    would write over tokens that are there."""
+    c = PagedKVCache(1, 8, 2, 64, page=8, max_seqs=2, max_len=32)
+    c.extend([5, 3])
+    old = _rand(8, 2, 64, dtype=F16, seed=1)
+    c.append(0, old, old)
+    c.extend([1, 1])
+    for n in (0, 2, 3):
+        k = _rand(2, 2, n, 64, dtype=F16, seed=2)
+        with pytest.raises(ValueError, match="append"):
+            c.append(0, k, k)
+    k = _rand(2, 2, 1, 64, dtype=F16, seed=3)
+    c.append(0, k, k)
+    got = c.read(0, 0)[0][0]
+    assert torch.equal(got[:, :5], old[:5].transpose(0, 1)) and torch.equal(got[:, 5], k[0, :, 0])
+    c.extend([2, 0])
+    for shape in ((2, 2, 1, 64), (2, 2, 2, 64)):                 # packed rows have three dimensions
+        with pytest.raises(ValueError, match="append"):
+            c.append(0, k.expand(shape), k.expand(shape))
+    c.check()
+
+
 # ---- gradients ----------------------------------------------------------------------------------
 
 def test_frequencies_and_tangents_are_refused():
