@@ -8,7 +8,6 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/AutogradState.h>
@@ -18,6 +17,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <limits>
 #include <string>
@@ -103,6 +103,106 @@ void refuse_grad(const char* who, std::initializer_list<const Tensor*> ts) {
     }
 }
 
+// ---- shared memory --------------------------------------------------------------------------
+// What a call writes must not be what it reads elsewhere, or another of its
+// outputs: the kernels' blocks run in no order.  A tensor is a set of runs of
+// `run` bytes at start + sum of index * step over its dimensions; two tensors
+// share memory if some difference of their runs' addresses is smaller than a run.
+struct Memory {
+    struct Dim {
+        int64_t n, step;                  // step > 0, in bytes; n > 1
+    };
+    int64_t start = 0, end = 0, run = 0;  // [start, end) holds every run
+    Dim dim[8];
+    int dims = 0;
+    bool repeats = false;                 // a step of 0: several indices at one address
+    explicit Memory(const Tensor& t) {
+        const int64_t item = (int64_t)t.element_size();
+        start = end = reinterpret_cast<int64_t>(t.data_ptr());
+        if (t.numel() == 0) return;
+        run = item;
+        if (t.is_contiguous()) {
+            run *= t.numel();
+        } else {
+            for (int64_t i = t.dim() - 1; i >= 0; --i) {
+                const int64_t n = t.size(i), step = t.stride(i) * item;
+                if (n == 1) continue;
+                if (step == run) run *= n;                // a longer run
+                else if (step == 0 || dims == 8) repeats = true;
+                else dim[dims++] = {n, step};
+            }
+        }
+        end += run;
+        for (int i = 0; i < dims; ++i) end += (dim[i].n - 1) * dim[i].step;
+    }
+};
+// Can base + sum x_i step_i, lo_i <= x_i <= hi_i, lie in (-below, above)?  Steps
+// descend, so of ordinary layouts few x_i are left at each.  `tries` bounds the
+// search; what is not found out counts as yes.
+struct Step {
+    int64_t step, lo, hi;
+};
+bool lands(int64_t base, const Step* d, int n, int64_t below, int64_t above, int& tries) {
+    if (--tries < 0) return true;
+    if (n == 0) return base > -below && base < above;
+    int64_t least = 0, most = 0;          // of the smaller steps
+    for (int i = 1; i < n; ++i) least += d[i].lo * d[i].step, most += d[i].hi * d[i].step;
+    const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t x0 = std::max(d->lo, floor_div(-below - base - most, d->step) + 1);
+    const int64_t x1 = std::min(d->hi, floor_div(above - base - least - 1, d->step));
+    for (int64_t x = x0; x <= x1; ++x)
+        if (lands(base + x * d->step, d + 1, n - 1, below, above, tries)) return true;
+    return false;
+}
+constexpr int kTries = 20000;
+void by_step(Step* d, int n) {
+    std::sort(d, d + n, [](const Step& a, const Step& b) { return a.step > b.step; });
+}
+bool share(const Memory& a, const Memory& b) {
+    if (a.end <= b.start || b.end <= a.start || a.run == 0 || b.run == 0) return false;
+    Step d[16];
+    int n = 0;
+    for (int i = 0; i < a.dims; ++i) d[n++] = {a.dim[i].step, 0, a.dim[i].n - 1};
+    for (int i = 0; i < b.dims; ++i) {
+        int j = 0;
+        while (j < n && d[j].step != b.dim[i].step) ++j;
+        if (j == n) d[n++] = {b.dim[i].step, 0, 0};
+        d[j].lo -= b.dim[i].n - 1;
+    }
+    by_step(d, n);
+    int tries = kTries;
+    return lands(a.start - b.start, d, n, a.run, b.run, tries);
+}
+// two indices of one tensor at the same memory
+bool folds(const Memory& a) {
+    if (a.repeats) return true;
+    Step d[8];
+    for (int i = 0; i < a.dims; ++i) d[i] = {a.dim[i].step, 0, a.dim[i].n - 1};
+    by_step(d, a.dims);
+    int tries = kTries;
+    for (int i = 0; i < a.dims; ++i) {    // the first step in which they differ
+        d[i].lo = 1;
+        for (int j = i + 1; j < a.dims; ++j) d[j].lo = -d[j].hi;
+        if (lands(0, d + i, a.dims - i, a.run, a.run, tries)) return true;
+    }
+    return false;
+}
+// An output that is `in` itself is written in place; any other overlap is a race.
+bool apart(const Tensor& out, const Tensor& in, bool same_is_fine) {
+    if (same_is_fine && out.data_ptr() == in.data_ptr()) {
+        bool same = true;
+        for (int64_t i = 0; same && i < out.dim(); ++i) same = out.size(i) == 1 || out.stride(i) == in.stride(i);
+        if (same) return true;
+    }
+    return !share(Memory(out), Memory(in));
+}
+bool apart_of(const Tensor& out, std::initializer_list<const Tensor*> ins) {
+    const Memory o(out);
+    for (const Tensor* t : ins)
+        if (t != nullptr && share(o, Memory(*t))) return false;
+    return true;
+}
+
 // 16-bit rows that the kernels can address: contiguous heads, 8-byte aligned,
 // strides of a multiple of 4 elements.  (B, H, S, D) or (tokens, H, D).
 struct Rows {
@@ -140,9 +240,7 @@ Rows out16(const char* who, const char* name, const Tensor& t, const Tensor& lik
             " is ", t.scalar_type(), " ", t.sizes(), " on ", t.device(), ", expected ", like.scalar_type(), " ",
             like.sizes(), " on cuda:", index);
     Rows r{t, {}};
-    bool ok = addressable(r.t, r.st);
-    for (int64_t i = 0; i < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) != 0);
-    require(ok, who, name, " must be 8-byte aligned rows that do not overlap, with strides of a multiple of 4 elements");
+    require(addressable(r.t, r.st) && !folds(Memory(t)), who, name, " must be 8-byte aligned rows that do not overlap, with strides of a multiple of 4 elements");
     return r;
 }
 // an output, straight from the CUDA allocator (through the dispatcher a call
@@ -158,14 +256,6 @@ Rows new16(const Tensor& like) {
            {}};
     addressable(r.t, r.st);
     return r;
-}
-// An output that is `in` itself is written in place; any other overlap is a race.
-// (Views that interleave, as q and k of packed rows, cannot be told apart
-// cheaply and pass.)
-bool apart(const Tensor& out, const Tensor& in, bool same_is_fine) {
-    if (same_is_fine && out.data_ptr() == in.data_ptr() && out.strides() == in.strides()) return true;
-    const auto st = at::get_overlap_status(out, in);
-    return st != at::MemOverlapStatus::Full && st != at::MemOverlapStatus::Partial;
 }
 const double* frequencies(const char* who, const Tensor& f, int index) {
     require(f.scalar_type() == at::kDouble && f.dim() == 1 && index_of(f) == index && f.is_contiguous(), who,
@@ -229,7 +319,8 @@ PyObject* rotary(PyObject* const* args) {
     if (q_out || k_out)
         require((!q_out || (apart(qo.t, qi.t, true) && (!k || apart(qo.t, ki.t, false)))) &&
                     (!k_out || (apart(ko.t, ki.t, true) && apart(ko.t, qi.t, false))) &&
-                    (!k || apart(qo.t, ko.t, false)),
+                    (!k || apart(qo.t, ko.t, false)) && (!q_out || apart_of(qo.t, {&pos, &f})) &&
+                    (!k_out || apart_of(ko.t, {&pos, &f})),
                 who, "out overlaps an input that it is not");
     copy3(sh.q_stride, qi.st);
     copy3(sh.q_out_stride, qo.st);
@@ -250,7 +341,7 @@ PyObject* rotary(PyObject* const* args) {
 // ---- the pages: k_pages, v_pages, table, lens, k_scale, v_scale, status -------------------------
 struct Pages {
     FkvPagedCache c = {};
-    const Tensor *k, *v, *k_scale, *v_scale;
+    const Tensor *k, *v, *k_scale, *v_scale, *table, *lens, *status;
     int index;
 };
 Pages pages(const char* who, PyObject* const* args, at::ScalarType dt) {
@@ -264,6 +355,9 @@ Pages pages(const char* who, PyObject* const* args, at::ScalarType dt) {
     p.v = &v;
     p.k_scale = ks;
     p.v_scale = vs;
+    p.table = &table;
+    p.lens = &lens;
+    p.status = status;
     const int index = p.index = index_of(k);
     const auto kind = k.scalar_type();
     require(index >= 0, who, "pages must be CUDA tensors");
@@ -345,8 +439,13 @@ PyObject* append(PyObject* const* args) {
         n.interleaved = truth(args[12]);
         n.amplitude = (float)number(args[13]);
     }
-    require(p.c.n_pages == 0 || (p.c.k_pages != p.c.v_pages && (!p.c.fp8 || p.c.k_scale != p.c.v_scale)), who,
-            "k_pages and v_pages (and their scales) must be different tensors");
+    const Memory into[4] = {Memory(*p.k), Memory(*p.v), Memory(p.c.fp8 ? *p.k_scale : *p.k),
+                            Memory(p.c.fp8 ? *p.v_scale : *p.v)};
+    const int parts = p.c.fp8 ? 4 : 2;
+    for (int i = 1; i < parts; ++i)
+        for (int j = 0; j < i; ++j)
+            require(!share(into[i], into[j]), who,
+                    "k_pages and v_pages (and their scales) must be different tensors that share no memory");
     require(q == nullptr || f != nullptr, who, "q is only rotated; pass inv_freq with it");
     require(q != nullptr || q_out == nullptr, who, "q_out without q");
     const c10::cuda::OptionalCUDAGuard guard(p.k->device());
@@ -361,10 +460,15 @@ PyObject* append(PyObject* const* args) {
         qo = q_out ? out16(who, "q_out", *q_out, *q, p.index) : new16(qi.t);
         if (q_out)
             require(apart(qo.t, qi.t, true) && apart(qo.t, kr.t, false) && apart(qo.t, vr.t, false) &&
-                        apart(qo.t, *p.k, false) && apart(qo.t, *p.v, false),
+                        apart_of(qo.t, {p.k, p.v, p.k_scale, p.v_scale, p.table, p.lens, p.status, cu, f}),
                     who, "q_out overlaps an input that it is not");
         n.q = qi.ptr();
         n.q_out = qo.ptr();
+    }
+    for (const Rows* r : std::initializer_list<const Rows*>{&kr, &vr, &qi}) {
+        if (!r->t.defined()) continue;
+        const Memory m(r->t);
+        for (int i = 0; i < parts; ++i) require(!share(m, into[i]), who, "k, v or q overlaps the pages or their scales");
     }
     n.k = kr.ptr();
     n.v = vr.ptr();
@@ -434,7 +538,7 @@ PyObject* attend(PyObject* const* args) {
         require(out.sizes() == q.sizes() && out.scalar_type() == dt && index_of(out) == p.index && out.is_contiguous() &&
                     (reinterpret_cast<uintptr_t>(out.data_ptr()) & 15) == 0,
                 who, "out must be a contiguous, 16-byte aligned tensor like q");
-        require(apart(out, q, false) && apart(out, *p.k, false) && apart(out, *p.v, false), who,
+        require(apart_of(out, {&q, p.k, p.v, p.k_scale, p.v_scale, p.table, p.lens, p.status}), who,
                 "out overlaps an input");
     }
     Tensor lse, ws;
@@ -451,6 +555,13 @@ PyObject* attend(PyObject* const* args) {
     PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));
     PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(lse));
     return r;
+}
+
+// share_memory(a, b): what the calls above refuse; b None: two indices of a
+PyObject* share_memory(PyObject* const* args) {
+    const char* who = "share_memory";
+    const Tensor &a = tensor(args[0], who, "a"), *b = maybe(args[1], who, "b");
+    return PyBool_FromLong(b ? share(Memory(a), Memory(*b)) : folds(Memory(a)));
 }
 
 template <PyObject* (*F)(PyObject* const*), int N>
@@ -504,6 +615,7 @@ PyMethodDef methods[] = {
     {"paged_append", FAST((&entry<append, 15>))},
     {"paged_read", FAST((&entry<read, 9>))},
     {"paged_attend", FAST((&entry<attend, 12>))},
+    {"share_memory", FAST((&entry<share_memory, 2>))},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fkv_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -51,7 +51,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     (B + 1,) int32: packed rows (T, Hk, D), sequence b's are
     [cu_new[b], cu_new[b + 1]), rows behind the last are padding.  The new
     tokens are the last of their sequences (``lens`` counts them), and two
-    sequences must not be given the same page to write.
+    sequences must not be given the same page to write.  k, v and q must share
+    no memory with the pages or their scales, q_out with nothing but q.
 
     With inv_freq the keys are rotated by their positions before they are
     stored (``apply_rotary``'s arguments), and so is q, which has k's layout
@@ -85,7 +86,7 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     out, of q's shape, and with return_lse the natural log-sum-exp of the
     scaled scores, (B, Hq) float32.  A sequence without tokens, or with none that
     has a page, gives zeros and -inf.  A score of +inf gives NaN and +inf; an infinite value gives a
-    non-finite output.  Lengths are read on the device, so the call can be
+    non-finite output.  ``out`` must share memory with nothing else.  Lengths are read on the device, so the call can be
     captured once and replayed as sequences grow within the table; neither they
     nor the table may change while it runs.  The work split follows the table's
     width and the lengths: the same inputs give the same bits, a wider table

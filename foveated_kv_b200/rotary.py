@@ -62,7 +62,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     ``amplitude``; the rest passes through.  ``inverse`` turns by the negative
     angles.  Angles are reduced to one turn in 64 bits, so far positions lose
     nothing.  Returns (q, k), or q alone without k: new tensors, or ``out``
-    (a tensor or pair of them, which may be the inputs themselves).
+    (a tensor or pair of them, which may be the inputs themselves; one that
+    shares memory with an input otherwise, or with itself, is refused).
     """
     qo, ko = (out, None) if out is None or isinstance(out, torch.Tensor) else out
     if out is not None and (qo is None or (ko is None) != (k is None)):

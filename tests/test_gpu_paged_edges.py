@@ -176,6 +176,57 @@ def test_cache_takes_one_row_per_slot():
     c.check()
 
 
+# ---- shared memory ------------------------------------------------------------------------------
+
+def test_outputs_that_share_memory_are_refused():
+    p, e = (R.Pages(8, [20, 100], 2, 64, 16, F16, fp8) for fp8 in (False, True))
+    f, pos = fkv.rotary_frequencies(64)[0], torch.arange(2, device="cuda")
+    qkv = _rand(2, 8, 64, dtype=F16)                             # packed rows: 4 q, 2 k, 2 v
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    other = lambda x: x.clone()
+    half = lambda x, n: x.view(-1).view(torch.uint8)[:n * 128].view(F16).view(2, -1, 64)    # its first rows as f16
+    store = torch.zeros(2 ** 14, dtype=F16, device="cuda")
+    folded = store.as_strided((2, 4, 64), (256, 32, 1))
+    far = torch.zeros(64, dtype=torch.int64, device="cuda")      # positions with rows of f16 over them
+    pool = torch.zeros(p.k_pages.shape[0] + 1, *p.k_pages.shape[1:], dtype=F16, device="cuda")
+    rotary = lambda **kw: fkv.apply_rotary(**dict(dict(q=q, k=k, positions=pos, inv_freq=f), **kw))
+    append = lambda p=p, **kw: fkv.paged_append(**dict(dict(k=k, v=v, q=q, inv_freq=f, **p.kw), **kw))
+    attend = lambda p=p, **kw: fkv.paged_attend(**dict(dict(q=other(q), **p.kw), **kw))
+    bad = [
+        lambda: rotary(out=(qkv[:, 1:5], other(k))), lambda: rotary(k=None, out=qkv[:, 1:5]),
+        lambda: rotary(out=(qkv[:, 2:6], other(k))), lambda: rotary(out=(other(q), qkv[:, 3:5])),
+        lambda: rotary(out=(folded, other(k))),
+        lambda: rotary(out=(store[:512].view(2, 4, 64), store[256:512].view(2, 2, 64))),
+        lambda: rotary(q=other(q)[:, :1], k=None, positions=far[:2], out=far.view(F16)[:128].view(2, 1, 64)),
+        lambda: rotary(q=other(q)[:, :1], k=None, out=f.view(F16)[:128].view(2, 1, 64)),
+        lambda: append(q_out=qkv[:, 1:5]), lambda: append(q_out=qkv[:, 2:6]), lambda: append(q_out=qkv[:, 4:]),
+        lambda: append(q_out=folded), lambda: append(k=half(p.k_pages, 4)), lambda: append(v=half(p.k_pages, 4)),
+        lambda: append(k=p.k_pages[:2, :, 3]), lambda: append(q=p.v_pages[:2, :, 3]),
+        lambda: append(e, k=half(e.v_scale, 4)), lambda: append(e, q_out=half(e.k_pages, 8)), lambda: append(e, q_out=half(e.k_scale, 8)),
+        lambda: append(k_pages=pool[1:], v_pages=pool[:-1]),
+        lambda: attend(q=q, out=q), lambda: attend(out=half(p.v_pages, 8)), lambda: attend(e, out=half(e.k_scale, 8)),
+        lambda: attend(e, out=half(e.v_pages, 8)),
+    ]
+    keep = [x.clone() for x in (qkv, p.k_pages.view(torch.int16), p.v_pages.view(torch.int16), e.k_scale.view(torch.int32))]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"case {i} was accepted")
+    for x, y in zip(keep, (qkv, p.k_pages.view(torch.int16), p.v_pages.view(torch.int16), e.k_scale.view(torch.int32))):
+        assert torch.equal(x, y)                                 # nothing ran
+    # what shares no memory still runs: beside each other in packed rows, in one store
+    want = rotary()
+    x = other(qkv)
+    got = fkv.apply_rotary(x[:, :4], x[:, 4:6], pos, f, out=(x[:, :4], x[:, 4:6]))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(x[:, 6:], v)
+    got = rotary(out=(store[:512].view(2, 4, 64), store[512:768].view(2, 2, 64)))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    append(k_pages=pool[:4], v_pages=pool[4:8], table=torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda"),
+           lens=torch.tensor([20, 30], dtype=torch.int32, device="cuda"))
+    assert torch.equal(pool[5, :, 3], v[0]) and torch.equal(pool[7, :, 13], v[1])
+    assert attend(out=store[:512].view(2, 4, 64)).data_ptr() == store.data_ptr()
+
+
 # ---- gradients ----------------------------------------------------------------------------------
 
 def test_frequencies_and_tangents_are_refused():

@@ -1,9 +1,12 @@
 """Host side of the paged cache's and rotary calls, without a GPU."""
 
+import random
+
 import pytest
 import torch
 
 import foveated_kv_b200 as fkv
+from foveated_kv_b200 import _native
 
 
 def _step():
@@ -30,3 +33,56 @@ def test_gradients_are_refused(name):
                 fkv.paged_append(**kw)
     with pytest.raises(ValueError, match="CUDA"):                # the tangent is gone with its level
         fkv.paged_append(**kw)
+
+
+def _places(t):
+    """Byte addresses of a tensor's elements, relative to its storage, with repeats."""
+    at = torch.tensor([t.storage_offset()])
+    for n, s in zip(t.shape, t.stride()):
+        at = (at[:, None] + torch.arange(n) * s).reshape(-1)
+    return (at[:, None] * t.element_size() + torch.arange(t.element_size())).reshape(-1).tolist()
+
+
+def test_shared_memory_of_random_views():
+    """The overlap test of the calls against the addresses themselves."""
+    rng, share = random.Random(1), _native.ops().share_memory
+    store = torch.zeros(400, dtype=torch.int32)
+    kinds = [0, 0]
+    for i in range(3000):
+        views = []
+        for j in range(2):
+            base = store if rng.random() < 0.7 else store.view(torch.int16)
+            dims = rng.randint(0, 4)
+            steps = [rng.choice([1, 2, 3, 4, 6, 8, 12, 16, 24, 40]) for _ in range(dims)]
+            if j and rng.random() < 0.5:
+                base, steps = first
+                dims = len(steps)
+            first = base, steps
+            shape = [rng.randint(1, 4) for _ in range(dims)]
+            if rng.random() < 0.03 and dims:
+                steps[0] = 0
+            if rng.random() < 0.02 and dims:
+                shape[-1] = 0
+            views.append(base.as_strided(shape, steps, rng.randint(0, 60)))
+        a, b = map(_places, views)
+        assert share(*views) == share(*views[::-1]) == bool(set(a) & set(b)), [(v.shape, v.stride(), v.storage_offset()) for v in views]
+        assert share(views[0], None) == (len(set(a)) < len(a)), [(v.shape, v.stride()) for v in views]
+        kinds[bool(set(a) & set(b))] += 1
+    assert min(kinds) > 500
+
+
+def test_shared_memory_of_packed_rows():
+    """Heads side by side in packed rows, however many: apart, and a view that is shifted: not."""
+    share = _native.ops().share_memory
+    qkv = torch.empty(100000, 48, 128, dtype=torch.float16)
+    q, k, v = qkv[:, :32], qkv[:, 32:40], qkv[:, 40:]
+    for a, b in ((q, k), (k, v), (v, q)):
+        assert not share(a, b) and not share(b, a)
+    assert share(qkv[:, 1:33], q) and share(qkv[:, 31:33], k) and not share(qkv[:, :32, :64], qkv[:, :32, 64:])
+    assert share(q[1:], q[:-1]) and not share(q[50000:], q[:50000])
+    t = qkv.view(10, 10000, 48, 128).transpose(1, 2)             # (B, H, S, D)
+    assert not share(t[:, :32], t[:, 32:]) and share(t[:, :33], t[:, 32:]) and not share(t, None)
+    assert not share(q, None) and not share(qkv[:, ::2], None)
+    assert share(qkv.view(-1).as_strided((100, 4, 128), (512, 64, 1)), None)   # heads of 128 every 64
+    assert share(qkv[:, :1].expand(-1, 4, -1), None)
+    assert not share(torch.empty(0), torch.empty(0)) and not share(torch.empty(0), None)
