@@ -95,7 +95,7 @@ int index_of(const Tensor& t) { return t.is_cuda() ? (int)t.get_device() : -1; }
 void refuse_grad(const char* who, std::initializer_list<const Tensor*> ts) {
     const bool back = at::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
     for (const Tensor* t : ts) {
-        if (t == nullptr) continue;
+        if (t == nullptr || t->unsafeGetTensorImpl()->autograd_meta() == nullptr) continue;
         require(!back || !t->requires_grad(), who,
                 "inputs that require a gradient are not supported (call it under torch.no_grad())");
         require(!forward || !t->_fw_grad(0).defined(), who,
