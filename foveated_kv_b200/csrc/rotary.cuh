@@ -58,8 +58,10 @@ constexpr int kEarlyBlocks = 148 * 4;
 // not move them over the stores of rows that could be the same memory
 constexpr int kRowsAtOnce = 4;
 
-// cosine and sine (times amplitude) of pair p at position pos
-__device__ __forceinline__ void rotary_pair(const double* __restrict__ inv_freq, int p, int64_t pos,
+// cosine and sine (times amplitude) of pair p at position pos (inv_freq without
+// __restrict__, which allows loads through the read-only cache: an early launch's
+// inputs may still be written while it waits)
+__device__ __forceinline__ void rotary_pair(const double* inv_freq, int p, int64_t pos,
                                             float amplitude, float& c, float& s) {
     constexpr double kInv2Pi = 0.15915494309189533577;
     const double turns = (double)pos * (inv_freq[p] * kInv2Pi);

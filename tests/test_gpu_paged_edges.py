@@ -227,6 +227,31 @@ def test_outputs_that_share_memory_are_refused():
     assert attend(out=store[:512].view(2, 4, 64)).data_ptr() == store.data_ptr()
 
 
+# ---- inputs written just before -----------------------------------------------------------------
+
+def test_frequencies_written_by_the_kernel_before():
+    """Small calls start beside their predecessor; what it writes is waited for."""
+    p = R.Pages(9, [20, 30], 2, 64, 16, F16, False)
+    q, k, pos = _rand(2, 4, 64, dtype=F16), _rand(2, 2, 64, dtype=F16), torch.arange(2, device="cuda") + 5
+    base = [fkv.rotary_frequencies(64, 10000.0 + 50 * i)[0] for i in range(40)]
+    want = [fkv.apply_rotary(q, None, pos, b) for b in base]
+    f = torch.zeros_like(base[0])
+    got = []
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for b in base:
+            f.copy_(b)
+            got.append(fkv.apply_rotary(q, None, pos, f))
+            f.mul_(0)
+            f.add_(b)
+            got.append(fkv.paged_append(k, k, q=q, inv_freq=f, **dict(p.kw, lens=(pos + 1).int(), table=p.table)))
+    for _ in range(5):
+        g.replay()
+        for i, x in enumerate(got):
+            assert torch.equal(x, want[i // 2]), i
+
+
 # ---- gradients ----------------------------------------------------------------------------------
 
 def test_frequencies_and_tangents_are_refused():
