@@ -12,6 +12,7 @@ using namespace fkvdev;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMostPairs = 4096;   // of a block: 32 KB of sines and cosines
 
 struct RotaryArgs {
     const uint16_t* q;
@@ -129,8 +130,8 @@ extern "C" int fkv_rotary(const FkvRotaryShape* sh, const uint16_t* q, const uin
     const int rows = kThreads / (sh->D / 8);
     const int passes = (std::max(sh->Hq, sh->Hk) + rows - 1) / rows;
     a.per_block = tokens_per_block(tokens, sh->Hq + sh->Hk);
-    // at most 512 pairs, and a row of each token at a time
-    while ((size_t)a.per_block * a.half * 2 * sizeof(float) > (32u << 10) || a.per_block > rows) a.per_block /= 2;
+    // a row of each token at a time, and sines within the limit
+    while (a.per_block * a.half > kMostPairs || a.per_block > rows) a.per_block /= 2;
     // few tokens: their heads are spread over more blocks
     const int gy = (int)std::min<int64_t>(passes, std::max<int64_t>(1, 592 / tokens));
     const dim3 grid((unsigned)((tokens + a.per_block - 1) / a.per_block), (unsigned)gy);
