@@ -1,6 +1,9 @@
 """Host side of the paged cache's and rotary calls, without a GPU."""
 
+import os
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -86,3 +89,20 @@ def test_shared_memory_of_packed_rows():
     assert share(qkv.view(-1).as_strided((100, 4, 128), (512, 64, 1)), None)   # heads of 128 every 64
     assert share(qkv[:, :1].expand(-1, 4, -1), None)
     assert not share(torch.empty(0), torch.empty(0)) and not share(torch.empty(0), None)
+
+
+CSRC = os.path.join(os.path.dirname(fkv.__file__), "csrc")
+
+
+def _make(*args):
+    r = subprocess.run(["make", "-C", CSRC, *args], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    return r.stdout
+
+
+def test_the_c_library_builds_without_torch():
+    """The default target wants nvcc alone, whatever the interpreter is."""
+    out = _make("-n", "-B", "PY=/bin/false")
+    assert "libfkv.so" in out and "ops.cpp" not in out and "torch" not in out
+    out = _make("-n", "-B", f"PY={sys.executable}", "python")
+    assert "libfkv.so" in out and "ops.cpp" in out and "-ltorch" in out
