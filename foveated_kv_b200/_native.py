@@ -181,6 +181,10 @@ def ops():
     if _ops is None:
         import importlib.machinery
         import importlib.util
+        import re
+        import sys
+
+        import torch
 
         lib = load()
         if not os.path.exists(OPS_PATH):
@@ -190,11 +194,15 @@ def ops():
             loader = importlib.machinery.ExtensionFileLoader("fkv_ops", OPS_PATH)
             mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("fkv_ops", loader))
             loader.exec_module(mod)
+            here = "torch {}.{}.{}, Python {}.{}".format(*re.findall(r"\d+", torch.__version__)[:3], *sys.version_info)
+            if mod.built_for != here:
+                raise ImportError(f"built for {mod.built_for}, this is {here}")
             mod.bind(FkvNativeError, *(C.cast(getattr(lib, n), P).value for n in (
                 "fkv_last_error", "fkv_rotary", "fkv_paged_append", "fkv_paged_read", "fkv_paged_attend",
                 "fkv_paged_attend_workspace_bytes")))
         except (ImportError, AttributeError) as e:
-            raise FkvNativeError(f"failed to load {OPS_PATH}: {e}") from e
+            raise FkvNativeError(f"failed to load {OPS_PATH}: {e}; rebuild it with "
+                                 "`python -m foveated_kv_b200.build`") from e
         _ops = mod
     return _ops
 

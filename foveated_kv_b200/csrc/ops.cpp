@@ -16,6 +16,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include <algorithm>
 #include <cmath>
@@ -622,4 +623,14 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "fkv_ops", nullptr, -1, methods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_fkv_ops() { return PyModule_Create(&module); }
+// with what it was built against, which the loader compares
+PyMODINIT_FUNC PyInit_fkv_ops() {
+    PyObject* m = PyModule_Create(&module);
+    const std::string made = c10::str("torch ", TORCH_VERSION_MAJOR, ".", TORCH_VERSION_MINOR, ".", TORCH_VERSION_PATCH,
+                                      ", Python ", PY_MAJOR_VERSION, ".", PY_MINOR_VERSION);
+    if (m != nullptr && PyModule_AddStringConstant(m, "built_for", made.c_str()) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import foveated_kv_b200 as fkv
-from foveated_kv_b200 import _native
+from foveated_kv_b200 import FkvNativeError, _native
 
 
 def _step():
@@ -106,3 +106,29 @@ def test_the_c_library_builds_without_torch():
     assert "libfkv.so" in out and "ops.cpp" not in out and "torch" not in out
     out = _make("-n", "-B", f"PY={sys.executable}", "python")
     assert "libfkv.so" in out and "ops.cpp" in out and "-ltorch" in out
+
+
+def test_the_python_calls_are_rebuilt_for_another_torch(tmp_path):
+    """fkv_ops.so is out of date when the interpreter or its torch is another one."""
+    ops, abi, ran = tmp_path / "fkv_ops.so", tmp_path / "python_abi", tmp_path / "ran"
+    compiler = f"touch {ran}; touch {ops}; true"                 # in the compiler's place
+
+    def rebuilt():
+        ran.unlink(missing_ok=True)
+        _make(str(ops), f"OPS={ops}", f"BUILD={tmp_path}", f"PY={sys.executable}", f"GXX={compiler}")
+        return ran.exists()
+
+    assert rebuilt() and torch.__version__ in abi.read_text()
+    assert not rebuilt() and not rebuilt()
+    abi.write_text(abi.read_text().replace(torch.__version__, "1.0.0"))
+    assert rebuilt() and torch.__version__ in abi.read_text() and not rebuilt()
+
+
+def test_the_python_calls_refuse_another_torch(monkeypatch):
+    assert _native.ops().built_for.startswith("torch " + torch.__version__.split("+")[0])
+    monkeypatch.setattr(_native, "_ops", None)
+    monkeypatch.setattr(torch, "__version__", "99.1.0+other")
+    with pytest.raises(FkvNativeError, match="this is torch 99.1.0.*rebuild"):
+        _native.ops()
+    monkeypatch.undo()
+    assert _native.ops()
