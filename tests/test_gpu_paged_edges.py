@@ -78,6 +78,62 @@ def test_scores_all_minus_infinity(n, dtype):
         assert torch.isnan(out).all() and (lse == -INF).all()
 
 
+# ---- attention: shares of several waves ---------------------------------------------------------
+
+@pytest.mark.parametrize("G,Hk,D,lens,waves", [
+    (8, 8, 64, [200000], 2),                                     # a descriptor for each stream
+    (16, 4, 128, [600000], 2),
+    (8, 8, 64, [760000], 3),
+    (4, 8, 64, [400000, 77, 0, 300001, 80000], 3),
+    (8, 16, 64, [9000 - 37 * i for i in range(48)], 3),
+    (8, 16, 64, [4100 - 3 * i for i in range(100)], 3),          # a descriptor for each CTA
+])
+def test_shares_of_several_waves(G, Hk, D, lens, waves):
+    """8-bit pages and much work: falling shares, of the wave count that the
+    units of work make, with every token in exactly one of them."""
+    per_sm = 2 if G == 16 else 3
+    ctas = per_sm * torch.cuda.get_device_properties(0).multi_processor_count
+    each = sum(-(-n // 128) for n in lens) * Hk // ctas
+    assert {2: 24 <= each < 98, 3: each >= 102}[waves], each     # where two and three waves begin, with some room
+    p = R.Pages(10, lens, Hk, D, 64, BF16, True, k_scale=0.1)
+    B, Hq = len(lens), G * Hk
+    # scores all alike: the sum counts the tokens, the output is the mean value
+    q = torch.zeros(B, Hq, D, dtype=BF16, device="cuda")
+    out, lse = fkv.paged_attend(q, return_lse=True, **p.kw)
+    vs = p.sequences("v")
+    for b, n in enumerate(lens):
+        if n == 0:
+            assert (out[b] == 0).all() and (lse[b] == -INF).all()
+            continue
+        # sums of equal weights are exact; log2 of up to 2^35 and its product to a few steps of 2^-18; a unit is 1.6e-4
+        assert (lse[b].double() - math.log(n)).abs().max() < 2.0 ** -16
+        mean, mag = vs[b].mean(1).repeat_interleave(G, 0), vs[b].abs().mean(1).repeat_interleave(G, 0)
+        tol = (n / 16 + 64) * 2.0 ** -23 * mag + 2.0 ** -11 * mag
+        assert ((out[b].double() - mean).abs() <= 2.0 ** -8 * (mean.abs() + tol) + tol).all()
+    # one token that takes all the weight of a head, somewhere in each sequence, a place for each head
+    rng = torch.Generator().manual_seed(11)
+    raw = p.k_pages.view(torch.uint8)
+    want, live = torch.zeros(B, Hq, D, dtype=torch.float64, device="cuda"), []
+    for b, n in enumerate(lens):
+        if n < Hq:
+            continue
+        live.append(b)
+        at = torch.randperm(n, generator=rng)[:Hq].cuda()
+        head, j = torch.arange(Hq, device="cuda") // G, torch.arange(Hq, device="cuda") % G
+        ids, row = p.table[b, at // 64].long(), at % 64
+        raw[ids, head, row] = 0
+        raw[ids, head, row, j] = 0x7E                            # 448
+        p.k_scale[ids, head, row] = 40.0 / 448.0
+        want[b] = vs[b][head, at]
+        q[b, torch.arange(Hq), j] = 1.0
+    out, lse = fkv.paged_attend(q, scale=1.0, return_lse=True, **p.kw)
+    # the others' weight: under 2^20 e^(1 - 40) = 2^-36 of values up to 6
+    err = (out.double() - want)[live].abs()
+    assert (err <= (2.0 ** -8 + 2.0 ** -10) * want[live].abs() + 2.0 ** -30).all()
+    assert (lse[live] - 40.0).abs().max() < 2.0 ** -15
+    assert torch.equal(fkv.paged_attend(q, scale=1.0, **p.kw), out)
+
+
 # ---- attention: weights far below the largest ---------------------------------------------------
 
 @pytest.mark.parametrize("bits", [20, 25, 28])
