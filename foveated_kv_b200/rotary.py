@@ -22,8 +22,15 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional
       'ntk'     the base raised so that the slowest pair slows by ``factor``
       'yarn'    pairs that make fewer than ``slow_turns`` turns in
                 ``original_len`` positions slow by ``factor``, those with more
-                than ``fast_turns`` stay, the others in between; the amplitude
-                is 0.1 ln(factor) + 1 (Peng et al., 2023)
+                than ``fast_turns`` stay, and between them the share that stays
+                grows linearly with the number of turns; the amplitude is
+                0.1 ln(factor) + 1 (as printed in Peng et al., 2023)
+
+    Many checkpoints with YaRN were trained with another ramp under that name,
+    linear in the pair's index, that is in the logarithm of the turns: in the
+    pairs between, its frequencies differ from these by up to 56 % (128 elements,
+    base 10000, 4096 positions, factor 8).  For such a model compute its own
+    vector; every call takes any (rot / 2,) float64 tensor as ``inv_freq``.
     """
     if rot_dim < 8 or rot_dim % 8:
         raise ValueError(f"rotary_frequencies: rot_dim {rot_dim} is not a multiple of 8")

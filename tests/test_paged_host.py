@@ -1,5 +1,6 @@
 """Host side of the paged cache's and rotary calls, without a GPU."""
 
+import math
 import os
 import random
 import subprocess
@@ -132,3 +133,18 @@ def test_the_python_calls_refuse_another_torch(monkeypatch):
         _native.ops()
     monkeypatch.undo()
     assert _native.ops()
+
+
+@pytest.mark.parametrize("rot,base,length,factor,slow,fast", [(128, 10000.0, 4096, 8.0, 1.0, 32.0), (64, 1e6, 32768, 4.0, 2.0, 20.0)])
+def test_yarn_ramp_is_linear_in_the_turns(rot, base, length, factor, slow, fast):
+    """Pair by pair against the formula, the pairs between the two ends among them."""
+    f, amplitude = fkv.rotary_frequencies(rot, base, scaling="yarn", factor=factor, original_len=length,
+                                          slow_turns=slow, fast_turns=fast, device="cpu")
+    between = 0
+    for p in range(rot // 2):
+        plain = base ** (-2.0 * p / rot)
+        turns = length * plain / (2 * math.pi)
+        keep = min(1.0, max(0.0, (turns - slow) / (fast - slow)))
+        between += 0.0 < keep < 1.0
+        assert f[p].item() == pytest.approx(plain * keep + plain / factor * (1 - keep), rel=1e-12)
+    assert between > 5 and amplitude == pytest.approx(0.1 * math.log(factor) + 1)
