@@ -45,9 +45,12 @@ class DecodeShape(C.Structure):
 
 
 def _strides(*names):
-    """Fields of int64 strides (sequence, token, head), flat: ctypes fills them faster than arrays."""
+    """Fields of int64 strides (sequence, token, head)."""
     return [(f"{n}_{s}", C.c_int64) for n in names for s in ("seq", "tok", "head")]
 
+
+# The descriptors of the rotary and paged entry points, for callers of the C ABI
+# from Python; the package's own calls go through fkv_ops.so, which fills them in C++.
 
 class RotaryShape(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("B", "S", "Hq", "Hk", "D", "rot", "bf16", "interleaved",

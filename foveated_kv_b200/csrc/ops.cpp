@@ -2,8 +2,8 @@
 // arguments, the outputs and the descriptors in C++, since a decode step calls
 // them for every layer and the same in Python took longer than the kernels
 // (us a call, Python and ctypes / this file: rotary step of 64 sequences 13.2 /
-// 5.1, append step 17.5 / 5.3, short read 12.7 / 5.5, attention over 1K tokens
-// 16.0 / 7.3).  The kernels stay behind the C ABI: bind() gets the addresses of
+// 5.0, append step 17.5 / 5.3, short read 12.7 / 5.6, attention over 1K tokens
+// 16.0 / 7.4).  The kernels stay behind the C ABI: bind() gets the addresses of
 // libfkv's functions from _native.py.
 #include <Python.h>
 

@@ -81,16 +81,22 @@ def paged_attend(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
                  status: Optional[torch.Tensor] = None):
     """Attention of one new token per sequence over its pages.
 
-    q (B, Hq, D) or (B, Hq, 1, D), Hq a multiple of Hk; ``scale`` 1/sqrt(D) by
-    default; the pages' own scales are not negative; ``window`` > 0 attends the last ``window`` tokens only.  Returns
-    out, of q's shape, and with return_lse the natural log-sum-exp of the
-    scaled scores, (B, Hq) float32.  A sequence without tokens, or with none that
-    has a page, gives zeros and -inf.  A score of +inf gives NaN and +inf; an infinite value gives a
-    non-finite output.  ``out`` must share memory with nothing else.  Lengths are read on the device, so the call can be
-    captured once and replayed as sequences grow within the table; neither they
-    nor the table may change while it runs.  The work split follows the table's
-    width and the lengths: the same inputs give the same bits, a wider table
-    may round differently.
+    q (B, Hq, D) or (B, Hq, 1, D), Hq a multiple of Hk; ``scale`` is 1/sqrt(D) by
+    default and ``window`` > 0 attends the last ``window`` tokens only.  The
+    pages' own scales must not be negative.  Returns out, of q's shape, and with
+    return_lse the natural log-sum-exp of the scaled scores, (B, Hq) float32.
+
+    A sequence without tokens, or with none that has a page, gives zeros and
+    -inf.  A score of +inf gives NaN and +inf; scores that are all -inf give NaN
+    and -inf; an infinite value gives a non-finite output.  Beside float8 pages
+    the softmax weights are rounded to float16.  ``out`` must share memory with
+    nothing else.
+
+    Lengths are read on the device, so the call can be captured once and
+    replayed as sequences grow within the table; neither they nor the table may
+    change while it runs.  The work split follows the table's width and the
+    lengths: the same inputs give the same bits, a wider table may round
+    differently.
     """
     return _native.ops().paged_attend(k_pages, v_pages, table, lens, k_scale, v_scale, status, q, scale, window,
                                       return_lse, out)
