@@ -171,22 +171,23 @@ class PagedKVCache:
         need = [-(-n // self.page) - len(p) for n, p in zip(lens, self._pages)]
         if sum(need) > len(self._free):
             raise _native.FkvNativeError(f"extend: {sum(need)} pages needed, {len(self._free)} free")
-        at, ids = [], []
-        for s, m in enumerate(need):
-            for _ in range(m):
-                at.append(s * self.width + len(self._pages[s]))
-                ids.append(self._free.pop())
-                self._pages[s].append(ids[-1])
-        if at:
-            upd = self._send([at, ids], torch.int64)
-            self.table.view(-1)[upd[0]] = upd[1].to(_I32)
-        self._lens = lens
-        self._packed = max(counts) > 1
-        self._new_rows = sum(counts) if self._packed else self.max_seqs
+        at = [s * self.width + len(self._pages[s]) + i for s, m in enumerate(need) for i in range(m)]
+        ids = self._free[len(self._free) - len(at):][::-1]
         cu = [0]
         for c in counts:
             cu.append(cu[-1] + c)
-        self._state.copy_(self._send(lens + [n if c else 0 for n, c in zip(lens, counts)] + cu, _I32))
+        # the device first: if a copy fails, nothing is taken
+        upd = self._send([at, ids], torch.int64) if at else None
+        state = self._send(lens + [n if c else 0 for n, c in zip(lens, counts)] + cu, _I32)
+        if at:
+            self.table.view(-1)[upd[0]] = upd[1].to(_I32)
+        self._state.copy_(state)
+        for j, page in zip(at, ids):
+            self._pages[j // self.width].append(page)
+        del self._free[len(self._free) - len(at):]
+        self._lens = lens
+        self._packed = max(counts) > 1
+        self._new_rows = sum(counts) if self._packed else self.max_seqs
 
     def _send(self, values, dtype) -> torch.Tensor:
         """Host values on the device, without waiting for the stream."""

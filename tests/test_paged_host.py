@@ -148,3 +148,28 @@ def test_yarn_ramp_is_linear_in_the_turns(rot, base, length, factor, slow, fast)
         between += 0.0 < keep < 1.0
         assert f[p].item() == pytest.approx(plain * keep + plain / factor * (1 - keep), rel=1e-12)
     assert between > 5 and amplitude == pytest.approx(0.1 * math.log(factor) + 1)
+
+
+def test_a_step_that_fails_takes_nothing(monkeypatch):
+    """extend whose copy to the device fails leaves pages, lengths and the step as they were."""
+    c = fkv.PagedKVCache(1, 6, 2, 64, page=8, max_seqs=2, max_len=40, device="cpu")
+    send = lambda values, dtype: torch.tensor(values, dtype=dtype)      # without pinned memory
+    monkeypatch.setattr(c, "_send", send)
+    c.extend([9, 3])
+    for fails in (1, 2):                                                # the page numbers, the lengths
+        def broken(values, dtype, left=[fails]):
+            left[0] -= 1
+            if left[0] == 0:
+                raise RuntimeError("out of memory")
+            return send(values, dtype)
+        monkeypatch.setattr(c, "_send", broken)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            c.extend([20, 1])
+        assert c.free_pages == 3 and c.lengths == [9, 3] and c.lens.tolist() == [9, 3]
+    monkeypatch.setattr(c, "_send", send)
+    c.extend([20, 1])
+    rows = c.table.tolist()
+    assert c.lengths == [29, 4] and c.free_pages == 1
+    assert sorted(rows[0][:4] + rows[1][:1] + c._free) == list(range(6)) and rows[0][4] == rows[1][1] == -1
+    c.release(0)
+    assert c.free_pages == 5
