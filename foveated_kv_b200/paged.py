@@ -191,7 +191,7 @@ class PagedKVCache:
 
     def _send(self, values, dtype) -> torch.Tensor:
         """Host values on the device, without waiting for the stream."""
-        return torch.tensor(values, dtype=dtype, pin_memory=True).to(self.device, non_blocking=True)
+        return torch.tensor(values, dtype=dtype, device="cpu", pin_memory=True).to(self.device, non_blocking=True)
 
     def _check_slot(self, slot: int) -> None:
         if not 0 <= slot < self.max_seqs:

@@ -42,7 +42,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional
     amplitude = 1.0
     if scaling == "ntk":
         base = base * factor ** (rot_dim / (rot_dim - 2))
-    f = float(base) ** -(torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    f = float(base) ** -(torch.arange(0, rot_dim, 2, dtype=torch.float64, device="cpu") / rot_dim)
     if scaling == "linear":
         f = f / factor
     elif scaling == "yarn":

@@ -308,6 +308,23 @@ def test_frequencies_written_by_the_kernel_before():
             assert torch.equal(x, want[i // 2]), i
 
 
+def test_cache_under_a_default_device():
+    """torch.device as a context changes where host tensors are made, not the cache's own."""
+    f = fkv.rotary_frequencies(64, scaling="yarn", factor=4.0, original_len=512)
+    with torch.device("cuda"):
+        g = fkv.rotary_frequencies(64, scaling="yarn", factor=4.0, original_len=512)
+        assert torch.equal(f[0], g[0]) and f[1] == g[1]
+        c = PagedKVCache(1, 8, 2, 64, page=8, max_seqs=2, max_len=32, inv_freq=f[0])
+        c.extend([9, 3])
+        k = _rand(12, 2, 64, dtype=F16)
+        c.append(0, k, k, k)
+        c.extend([1, 1])
+        c.attend(0, c.append(0, k[:2], k[:2], k[:2]))
+        assert torch.equal(c.read(0, 0)[1][0, :, :9], k[:9].transpose(0, 1))
+        c.release(0)
+        c.check()
+
+
 # ---- gradients ----------------------------------------------------------------------------------
 
 def test_frequencies_and_tangents_are_refused():
